@@ -35,6 +35,8 @@ BINDINGS = {
     "spfa_local_2d_dilated": ("Sparse_FlashAttention_Local_2D_Dilated", "sp_flatt_local_2d_dilated.cpp"),
     "spfa_global_no_local": ("Sparse_FlashAttention_Global_No_Local", "sp_flatt_global_no_local.cpp"),
     "spfa_bigbird": ("Sparse_FlashAttention_BigBird", "sp_flatt_bigbird.cpp"),  # additive: the fused union of masks
+    "spfa_cache": ("Sparse_FlashAttention_Cache", "sp_flatt_cache.cpp"),  # additive: paged key / value caches
+    "spfa_tree": ("Sparse_FlashAttention_Tree", "sp_flatt_tree.cpp"),  # additive: drafted token trees over a cache
 }
 
 
@@ -135,6 +137,7 @@ def build_binding(name: str, force: bool = False) -> str:
     folder, src = BINDINGS[name]
     out = binding_path(name)
     deps = [os.path.join(HERE, folder, src), os.path.join(HERE, "bindings", "binding_common.h"),
+            os.path.join(HERE, "bindings", "cache_common.h"),
             os.path.join(INCLUDE, "spfa_b200.h")]
     if not force and _newer(out, deps):
         return out
@@ -146,7 +149,7 @@ def build_binding(name: str, force: bool = False) -> str:
 
 def build_all(force: bool = False, verbose: bool = False) -> dict[str, str]:
     out = {"libspfa_b200": build_lib(force, verbose)}
-    with ThreadPoolExecutor(max_workers=min(7, os.cpu_count() or 1)) as ex:
+    with ThreadPoolExecutor(max_workers=min(len(BINDINGS), os.cpu_count() or 1)) as ex:
         for name, path in zip(BINDINGS, ex.map(lambda n: build_binding(n, force), BINDINGS)):
             out[name] = path
     return out

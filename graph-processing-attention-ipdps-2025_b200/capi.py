@@ -40,6 +40,7 @@ EXPORTS = (
     "spfa_csr_forward_16", "spfa_csr_forward_16_ws", "spfa_csr_workspace_bytes_16", "spfa_coo_forward_16", "spfa_tiled_16_usable", "spfa_local_forward_tiled_16", "spfa_local_1d_dilated_forward_tiled_16", "spfa_local_forward_16", "spfa_local_1d_dilated_forward_16",
     "spfa_local_2d_dilated_forward_16", "spfa_global_no_local_workspace_bytes_16", "spfa_global_no_local_forward_16",
     "spfa_csr_workspace_bytes_idx32", "spfa_csr_forward_f32_idx32", "spfa_coo_forward_f32_idx32", "spfa_coo_plan_build_idx32",
+    "spfa_cache_append", "spfa_cache_read", "spfa_cache_keep", "spfa_tree_workspace_bytes", "spfa_tree_forward",
 )
 
 _lib = None
@@ -147,6 +148,16 @@ def lib() -> ctypes.CDLL:
     L.spfa_coo_static_max_rows.restype = i64
     L.spfa_coo_forward_f32_static.restype = i32
     L.spfa_coo_forward_f32_static.argtypes = [vp] * 5 + [i64] + [vp] * 3 + [i64, i64, i64, i32, i32, vp]
+    L.spfa_cache_append.restype = i32
+    L.spfa_cache_append.argtypes = [vp, i32, vp, vp, vp, vp, vp, i64, vp]
+    L.spfa_cache_read.restype = i32
+    L.spfa_cache_read.argtypes = L.spfa_cache_append.argtypes
+    L.spfa_cache_keep.restype = i32
+    L.spfa_cache_keep.argtypes = [vp, vp, i64, vp, vp]
+    L.spfa_tree_workspace_bytes.restype = sz
+    L.spfa_tree_workspace_bytes.argtypes = [vp, i32, i64, i64]
+    L.spfa_tree_forward.restype = i32
+    L.spfa_tree_forward.argtypes = [vp, i32, vp, vp, vp, i64, i64, vp, i64, vp, vp, vp, vp, i32, vp, sz, vp]
     for name in ("spfa_local", "spfa_local_1d_dilated", "spfa_local_2d_dilated"):
         f = getattr(L, name + "_workspace_bytes")
         f.restype = sz
@@ -507,6 +518,135 @@ def forward_16(kind, Q, K, V, m, l, O, *, p0=0, p1=0, global_inds=None, row_off=
             else:
                 raise ValueError(kind)
         check(rc)
+    return O
+
+
+class KvCache(ctypes.Structure):
+    """spfa_kv_cache of include/spfa_b200.h."""
+    _fields_ = [("K", ctypes.c_void_p), ("V", ctypes.c_void_p), ("K_scale", ctypes.c_void_p), ("V_scale", ctypes.c_void_p),
+                ("K_stride", ctypes.c_int64 * 3), ("V_stride", ctypes.c_int64 * 3),
+                ("K_scale_stride", ctypes.c_int64 * 3), ("V_scale_stride", ctypes.c_int64 * 3),
+                ("n_pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("n_heads", ctypes.c_int64),
+                ("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("n_seq", ctypes.c_int64),
+                ("table_width", ctypes.c_int64), ("d", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+ROWS_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+CACHE_CODE = {**ROWS_CODE, torch.float8_e4m3fn: 3, torch.int8: 4}
+
+
+def kv_cache(K_pages, V_pages, page_table, lens, K_scale=None, V_scale=None) -> KvCache:
+    """Describe a paged cache: pages [n_pages, page_size, heads, d] (float32, float16, bfloat16, float8_e4m3fn or int8; last
+    dimension contiguous), page_table [sequences, pages] and lens [sequences] int32, and for the 8-bit types the scales
+    [n_pages, page_size, heads] float32. The description holds addresses: the tensors have to outlive it."""
+    dev = K_pages.device
+    if not K_pages.is_cuda:
+        raise SpfaError(-1, "tensors must be CUDA tensors (there is no CPU path)")
+    if K_pages.dtype not in CACHE_CODE or K_pages.dim() != 4 or V_pages.shape != K_pages.shape or V_pages.dtype != K_pages.dtype:
+        raise SpfaError(-1, "K_pages and V_pages must be [n_pages, page_size, heads, d] of one cache dtype")
+    if (K_pages.stride(3) != 1 or V_pages.stride(3) != 1) and K_pages.shape[3] != 1:
+        raise SpfaError(-1, "the last dimension of the pages must be contiguous")
+    quantised = CACHE_CODE[K_pages.dtype] >= 3
+    if (K_scale is not None) != quantised or (V_scale is not None) != quantised:
+        raise SpfaError(-1, "K_scale and V_scale belong to 8-bit caches, and only to them")
+    _i32(dev, page_table=page_table, lens=lens)
+    if page_table.dim() != 2 or lens.dim() != 1 or page_table.shape[0] != lens.shape[0]:
+        raise SpfaError(-1, "page_table [sequences, pages] and lens [sequences] must have one row per sequence")
+    for t in (V_pages,) + ((K_scale, V_scale) if quantised else ()):
+        if t.device != dev:
+            raise SpfaError(-1, "the tensors of a cache must be on one device")
+    c = KvCache()
+    c.K, c.V = K_pages.data_ptr(), V_pages.data_ptr()
+    c.K_stride[:], c.V_stride[:] = K_pages.stride()[:3], V_pages.stride()[:3]
+    if quantised:
+        for t in (K_scale, V_scale):
+            if t.dtype != torch.float32 or t.shape != K_pages.shape[:3]:
+                raise SpfaError(-1, "K_scale and V_scale must be float32 [n_pages, page_size, heads]")
+        c.K_scale, c.V_scale = K_scale.data_ptr(), V_scale.data_ptr()
+        c.K_scale_stride[:], c.V_scale_stride[:] = K_scale.stride(), V_scale.stride()
+    c.n_pages, c.page_size, c.n_heads, c.d = K_pages.shape
+    c.page_table, c.lens = page_table.data_ptr(), lens.data_ptr()
+    c.n_seq, c.table_width = page_table.shape
+    c.dtype = CACHE_CODE[K_pages.dtype]
+    return c
+
+
+def _i32(dev, **ts):
+    for name, t in ts.items():
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev:
+            raise SpfaError(-1, f"{name} must be a contiguous torch.int32 tensor on the cache's device")
+
+
+def _rows3(dev, cache, heads, *ts):
+    """dtype code of rows [n, heads, d] whose last dimension is contiguous."""
+    for t in ts:
+        if t.device != dev or t.dtype != ts[0].dtype or t.dtype not in ROWS_CODE:
+            raise SpfaError(-1, "rows must be float32, float16 or bfloat16 tensors of one dtype on the cache's device")
+        if tuple(t.shape) != (ts[0].shape[0], heads, cache.d) or (t.stride(2) != 1 and t.shape[2] != 1):
+            raise SpfaError(-1, f"rows must be [n, {heads}, {cache.d}] with a contiguous last dimension")
+    return ROWS_CODE[ts[0].dtype]
+
+
+def _strides(t):
+    return (ctypes.c_int64 * 2)(*t.stride()[:2])
+
+
+def _cu(dev, cache, cu_rows):
+    _i32(dev, cu_rows=cu_rows)
+    if tuple(cu_rows.shape) != (cache.n_seq + 1,):
+        raise SpfaError(-1, "cu_rows must have one entry more than there are sequences")
+    return _ptr(cu_rows)
+
+
+def cache_append(cache: KvCache, K, V, cu_rows):
+    """Write the rows K, V [n, heads, d] to their positions in the cache, in its type."""
+    dev = cu_rows.device
+    code = _rows3(dev, cache, cache.n_heads, K, V)
+    with torch.cuda.device(dev):
+        if K.shape[0] and cache.n_seq:
+            check(lib().spfa_cache_append(ctypes.byref(cache), code, _ptr(K), _strides(K), _ptr(V), _strides(V),
+                                          _cu(dev, cache, cu_rows), K.shape[0], _stream(dev)))
+
+
+def cache_read(cache: KvCache, K, V, cu_rows):
+    """Fill the rows K, V [n, heads, d] from their positions in the cache."""
+    dev = cu_rows.device
+    code = _rows3(dev, cache, cache.n_heads, K, V)
+    with torch.cuda.device(dev):
+        if K.shape[0] and cache.n_seq:
+            check(lib().spfa_cache_read(ctypes.byref(cache), code, _ptr(K), _strides(K), _ptr(V), _strides(V),
+                                        _cu(dev, cache, cu_rows), K.shape[0], _stream(dev)))
+    return K, V
+
+
+def cache_keep(cache: KvCache, kept, n_kept):
+    """Move position lens[b] + kept[b, i] to lens[b] + i for i < n_kept[b]; kept is ascending."""
+    dev = kept.device
+    _i32(dev, kept=kept, n_kept=n_kept)
+    if kept.dim() != 2 or kept.shape[0] != cache.n_seq or tuple(n_kept.shape) != (cache.n_seq,):
+        raise SpfaError(-1, "kept [sequences, width] and n_kept [sequences] must have one row per sequence")
+    with torch.cuda.device(dev):
+        if kept.numel():
+            check(lib().spfa_cache_keep(ctypes.byref(cache), _ptr(kept), kept.shape[1], _ptr(n_kept), _stream(dev)))
+
+
+def tree_forward(cache: KvCache, Q, cu_rows, tree_mask, m, l, O, first=False):
+    """Attention of the drafted rows Q [n, query heads, d] over the cache (include/spfa_b200.h: spfa_tree_forward)."""
+    dev = cu_rows.device
+    n, heads = Q.shape[:2]
+    code = _rows3(dev, cache, heads, Q, O)
+    if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.dim() != 2 or tree_mask.shape[0] != n \
+            or not tree_mask.is_contiguous() or tree_mask.device != dev:
+        raise SpfaError(-1, "tree_mask must be a contiguous torch.bool / torch.uint8 tensor [rows, drafted positions]")
+    for t in (m, l):
+        if t.dtype != torch.float32 or tuple(t.shape) != (n, heads) or not t.is_contiguous() or t.device != dev:
+            raise SpfaError(-1, "m and l must be contiguous float32 tensors [rows, query heads]")
+    with torch.cuda.device(dev):
+        if n and cache.n_seq:
+            buf, wp, wb = workspace(lib().spfa_tree_workspace_bytes(ctypes.byref(cache), code, n, heads), dev)
+            check(lib().spfa_tree_forward(ctypes.byref(cache), code, _ptr(Q), _strides(Q), _cu(dev, cache, cu_rows), n, heads,
+                                          _ptr(tree_mask), tree_mask.shape[1], _ptr(m), _ptr(l), _ptr(O), _strides(O), int(first),
+                                          wp, wb, _stream(dev)))
     return O
 
 

@@ -1,0 +1,98 @@
+// C ABI of the attention of drafted token trees over a paged cache. Declared in include/spfa_b200.h.
+#include <cmath>
+
+#include "tree_launch.cuh"
+
+namespace spfa {
+namespace {
+
+constexpr int kCtas = 296;  // of the context kernel: two on each of 148 SMs
+
+struct TreeLayout {
+  int row_tile, d_pad;
+  int64_t rows;
+  size_t cut, ml, O, total;
+};
+TreeLayout tree_layout(const spfa_kv_cache* c, int64_t n_rows, int64_t n_q_heads) {
+  TreeLayout t{};
+  t.row_tile = tree::kAnyRows;
+  t.d_pad = (c->d + 3) / 4 * 4;
+  t.rows = n_rows * n_q_heads + (int64_t)t.row_tile * kCtas;
+  t.cut = 0;
+  t.ml = align_up((size_t)(c->n_seq + 1) * 8);
+  t.O = t.ml + align_up((size_t)t.rows * 8);
+  t.total = t.O + align_up((size_t)t.rows * t.d_pad * 4);
+  return t;
+}
+
+int check_tree(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
+  const int rc = check_cache(c, dtype);
+  if (rc != SPFA_OK) return rc;
+  if (n_rows < 0 || n_q_heads < 1 || n_q_heads % c->n_heads) return SPFA_ERR_BAD_ARG;
+  if (n_rows > kMost32 || n_q_heads > 65535 || n_rows * n_q_heads > kMost32) return SPFA_ERR_TOO_LARGE;
+  return SPFA_OK;
+}
+
+}  // namespace
+}  // namespace spfa
+
+using namespace spfa;
+
+extern "C" {
+
+size_t spfa_tree_workspace_bytes(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
+  return check_tree(c, dtype, n_rows, n_q_heads) == SPFA_OK ? tree_layout(c, n_rows, n_q_heads).total : 0;
+}
+
+int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride, const int32_t* cu_rows,
+                      int64_t n_rows, int64_t n_q_heads, const uint8_t* tree_mask, int64_t mask_width, float* m, float* l, void* O,
+                      const int64_t* O_stride, int first, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_tree(c, dtype, n_rows, n_q_heads);
+  if (rc != SPFA_OK) return rc;
+  const int size = dtype_bytes(dtype);
+  if (!Q || !Q_stride || !cu_rows || !m || !l || !O || !O_stride || mask_width < 0 || (mask_width > 0 && !tree_mask)) return SPFA_ERR_BAD_ARG;
+  if (!aligned_to(Q, size) || !aligned_to(O, size) || !aligned4(cu_rows) || !aligned4(m) || !aligned4(l)) return SPFA_ERR_BAD_ARG;
+  if (Q_stride[0] < 0 || Q_stride[1] < 0 || O_stride[0] < 0 || O_stride[1] < 0) return SPFA_ERR_BAD_ARG;
+  const TreeLayout t = tree_layout(c, n_rows, n_q_heads);
+  rc = check_workspace(workspace, workspace_bytes, t.total);
+  if (rc != SPFA_OK) return rc;
+  if (n_rows == 0 || c->n_seq == 0) return SPFA_OK;
+
+  tree::Call a{};
+  a.c = cache_view(c);
+  a.Q = static_cast<const char*>(Q);
+  a.q_stride[0] = Q_stride[0];
+  a.q_stride[1] = Q_stride[1];
+  a.cu_rows = cu_rows;
+  a.n_rows = n_rows;
+  a.n_q_heads = (int32_t)n_q_heads;
+  a.group = (int32_t)(n_q_heads / c->n_heads);
+  a.scale_log2e = (1.0f / sqrtf((float)c->d)) * kLog2e;
+  a.row_tile = t.row_tile;
+  a.tile_keys = tree::any_tile_keys(c->d);
+  a.page_tiles = 0;
+  a.least = 1;
+  a.n_cta = kCtas;
+  char* ws = static_cast<char*>(workspace);
+  a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
+  a.ml = reinterpret_cast<float2*>(ws + t.ml);
+  a.O = reinterpret_cast<float*>(ws + t.O);
+  a.d_pad = t.d_pad;
+  tree::MergeArgs g{};
+  g.mask = tree_mask;
+  g.mask_width = mask_width;
+  g.m = m;
+  g.l = l;
+  g.O = static_cast<char*>(O);
+  g.o_stride[0] = O_stride[0];
+  g.o_stride[1] = O_stride[1];
+  g.first = first ? 1 : 0;
+  const bool vec = cache_rows_align(c, 4) && rows_align(Q, Q_stride, size, 4) && rows_align(O, O_stride, size, 4);
+  cudaStream_t st = (cudaStream_t)stream;
+  g_last_path.store(SPFA_PATH_GATHER);
+  if (dtype == SPFA_DTYPE_F16) return tree::launch_f16(c, a, g, vec, st);
+  if (dtype == SPFA_DTYPE_BF16) return tree::launch_bf16(c, a, g, vec, st);
+  return tree::launch_f32(c, a, g, vec, st);
+}
+
+}  // extern "C"

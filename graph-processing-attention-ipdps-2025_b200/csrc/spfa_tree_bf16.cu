@@ -1,0 +1,12 @@
+// Tree attention with Q and O of type __nv_bfloat16.
+#include "tree_launch.cuh"
+
+namespace spfa {
+namespace tree {
+
+int launch_bf16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
+  return launch_by_cache<__nv_bfloat16>(c, a, g, vec, st);
+}
+
+}  // namespace tree
+}  // namespace spfa

@@ -1,0 +1,598 @@
+// Attention of drafted token trees over a paged cache.
+//
+// Row i of sequence b (one query head of one drafted token) sees every committed key [0, len_b) and, of the drafted rows, the
+// keys len_b + j that tree_mask names. That is a dense part and a few entries, and they are computed apart:
+//
+//   context kernel  softmax partials over the committed keys. All rows see all of them, so there is no mask; the g query heads
+//                   of a key head and the tokens of a sequence are the rows of one product. (b, key head, row tile) is a unit;
+//                   the units' key tiles, one after the other, are one long list that is cut evenly over the CTAs of one
+//                   wave, whatever the lengths are: lens and cu_rows are read on the device. A piece (unit x CTA) leaves an
+//                   un-normalised O row with its maximum and sum in the workspace.
+//   merge kernel    one warp per row: the drafted keys that its mask names, its pieces, the incoming (m, l, O), and the store.
+//
+// Scores are kept in units of log2: s2 = (q . k) log2(e) / sqrt(d).
+#pragma once
+#include "cache_common.cuh"
+#include "spfa_common.cuh"
+
+namespace spfa {
+namespace tree {
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+struct Call {
+  CacheView c;
+  const char* Q;
+  int64_t q_stride[2];  // elements from row to row, head to head
+  const int32_t* cu_rows;
+  int64_t n_rows;
+  int32_t n_q_heads, group;  // group = query heads of a key head
+  float scale_log2e;
+  // cutting the list of key tiles
+  int32_t row_tile, tile_keys;  // rows of a unit, keys of a tile
+  int32_t page_tiles;           // tiles of a page (pages of tile_keys positions and more), 0: a tile spans whole pages
+  int32_t least;                // key tiles that a CTA takes at least
+  int32_t n_cta;                // grid of the context kernel
+  // workspace
+  int64_t* cut;   // [0]: tiles per CTA, [1 + b]: first tile of sequence b in the list
+  float2* ml;     // maximum and sum of a piece's row
+  float* O;       // [rows][d_pad]
+  int32_t d_pad;
+
+  __device__ __forceinline__ int64_t tiles_of(int64_t len) const {
+    if (page_tiles == 0) return (len + tile_keys - 1) / tile_keys;
+    const int64_t full = len / c.page_size, rest = len - full * c.page_size;
+    return full * page_tiles + (rest + tile_keys - 1) / tile_keys;
+  }
+  __device__ __forceinline__ int64_t row_tiles(int64_t tokens) const { return (tokens * group + row_tile - 1) / row_tile; }
+  // Key tiles of all units of sequence b.
+  __device__ __forceinline__ int64_t weight(int32_t b) const {
+    int64_t begin, end;
+    rows_of(cu_rows, b, n_rows, begin, end);
+    return end == begin ? 0 : tiles_of(c.len_of(b)) * row_tiles(end - begin) * c.n_heads;
+  }
+  // First partial row of local row x of key head h in CTA `cta`: rows of a sequence lie together, the CTAs of a row row_tile
+  // apart. Pieces follow each other with growing unit or growing CTA, so no two of them meet.
+  __device__ __forceinline__ int64_t partial_row(int64_t begin, int64_t tokens, int32_t h, int64_t x, int64_t cta) const {
+    return begin * n_q_heads + (int64_t)h * tokens * group + x + cta * row_tile;
+  }
+};
+
+struct Cut {  // what block_cut leaves in shared memory
+  int64_t first, last;  // this CTA's key tiles in the list
+  int64_t start;        // first tile of sequence b
+  int32_t b;
+  int32_t warp_sum_at;  // (padding)
+  int64_t warp_sum[32];
+};
+
+// Finds this CTA's share of the list (all NT threads). CTA 0 leaves the starts of the sequences for the merge kernel.
+template <int NT>
+__device__ __forceinline__ void block_cut(const Call& a, Cut* s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t n_seq = a.c.n_seq;
+  int64_t own = 0;  // of sequence threadIdx.x; kept, as most calls have no more sequences than threads
+  int64_t sum = 0;
+  for (int32_t b = threadIdx.x; b < n_seq; b += NT) {
+    const int64_t w = a.weight(b);
+    if (b == (int32_t)threadIdx.x) own = w;
+    sum += w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+  if (lane == 0) s->warp_sum[warp] = sum;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) total += s->warp_sum[w];
+  int64_t chunk = (total + a.n_cta - 1) / a.n_cta;
+  if (chunk < a.least) chunk = a.least;
+  const int64_t first = (int64_t)blockIdx.x * chunk;
+  if (threadIdx.x == 0) {
+    s->first = first < total ? first : total;
+    s->last = first + chunk < total ? first + chunk : total;
+    s->b = n_seq;
+    if (blockIdx.x == 0) a.cut[0] = chunk;
+  }
+  __syncthreads();
+  int64_t base = 0;
+  for (int32_t b0 = 0; b0 < n_seq; b0 += NT) {
+    const int32_t b = b0 + (int32_t)threadIdx.x;
+    const int64_t w = b0 == 0 ? own : (b < n_seq ? a.weight(b) : 0);
+    int64_t x = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(kFullMask, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s->warp_sum[warp] = x;
+    __syncthreads();
+    int64_t before = base;
+    for (int w2 = 0; w2 < NT / 32; ++w2) {
+      if (w2 < warp) before += s->warp_sum[w2];
+      base += s->warp_sum[w2];
+    }
+    const int64_t start = before + x - w;
+    if (blockIdx.x == 0 && b < n_seq) a.cut[1 + b] = start;
+    if (w > 0 && s->first >= start && s->first < start + w) {  // one thread at most
+      s->b = b;
+      s->start = start;
+    }
+    __syncthreads();
+  }
+}
+
+// Walks the pieces of a CTA: piece = consecutive key tiles [t0, t0 + n) of one unit. Every role of a CTA walks on its own.
+struct Walk {
+  int64_t at, last, start, weight, begin, tokens, len, tiles;
+  int32_t b, h;
+  int64_t row0;  // first row of the unit's row tile among the tokens * group rows of the key head
+  int64_t t0, n;
+
+  __device__ __forceinline__ void open(const Call& a) {
+    int64_t end;
+    rows_of(a.cu_rows, b, a.n_rows, begin, end);
+    tokens = end - begin;
+    len = a.c.len_of(b);
+    tiles = a.tiles_of(len);
+    weight = tokens ? tiles * a.row_tiles(tokens) * a.c.n_heads : 0;
+  }
+  __device__ __forceinline__ void init(const Call& a, const Cut* s) {
+    at = s->first;
+    last = s->last;
+    b = s->b;
+    start = s->start;
+    n = 0;
+    if (at < last) open(a);
+  }
+  // The next piece; false behind the last one.
+  __device__ __forceinline__ bool next(const Call& a) {
+    at += n;
+    if (at >= last) return false;
+    while (at >= start + weight) {  // ends: `at` is below the list's total
+      start += weight;
+      ++b;
+      open(a);
+    }
+    const int64_t u = (at - start) / tiles;
+    t0 = (at - start) - u * tiles;
+    n = tiles - t0 < last - at ? tiles - t0 : last - at;
+    const int64_t rt = a.row_tiles(tokens);
+    h = (int32_t)(u / rt);
+    row0 = (u - (int64_t)h * rt) * a.row_tile;
+    return true;
+  }
+};
+
+// ---- context kernel without tensor cores: 32-bit products, any types and any d ---------------------------------------------
+//
+// 256 threads, 16 rows, TK keys at a time in shared memory as 32-bit values. Scores: a warp takes 16 keys and a slice of d, each
+// thread 4 rows x 2 keys, so that six 16-byte shared loads feed 32 products a lane. P V: a thread owns 4 rows x 4 columns of O in
+// registers and, where d leaves threads over, a share of the keys.
+template <int DP>
+struct PlanAny {
+  static constexpr int kThreads = 256, kRows = 16;
+  static constexpr int TK = DP <= 128 ? 64 : (DP == 256 ? 32 : 16);
+  static constexpr int KB = TK / 16, DS = 8 / KB;  // key blocks x slices of d = 8 warps
+  static constexpr int CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (4 * CGT);
+  static constexpr int kPitch = DP + 4;  // floats: rows start 16 bytes further round the banks
+  static constexpr int kOffQ = 0, kOffK = kOffQ + kRows * kPitch * 4, kOffV = kOffK + TK * kPitch * 4;
+  static constexpr int kOffS = kOffV + TK * kPitch * 4, kOffP = kOffS + DS * kRows * TK * 4, kOffRow = kOffP + TK * 20 * 4;
+  static constexpr int kOffKey = kOffRow + 3 * kRows * 4, kOffCut = kOffKey + TK * 24, kBytes = kOffCut + (int)sizeof(Cut);
+  static_assert(KS * kRows * DP <= (TK * kPitch) * 2, "the shares of O are added up where K and V were");
+};
+
+template <int DP, class TQ, class TC>
+__global__ void __launch_bounds__(256) context_any_kernel(const Call a, const int vec) {
+  using P = PlanAny<DP>;
+  constexpr int TK = P::TK, R = P::kRows, PITCH = P::kPitch;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* Qs = reinterpret_cast<float*>(smem + P::kOffQ);
+  float* Ks = reinterpret_cast<float*>(smem + P::kOffK);
+  float* Vs = reinterpret_cast<float*>(smem + P::kOffV);
+  float* Ss = reinterpret_cast<float*>(smem + P::kOffS);
+  float* Ps = reinterpret_cast<float*>(smem + P::kOffP);  // [key][20]
+  float* row_m = reinterpret_cast<float*>(smem + P::kOffRow);
+  float* row_l = row_m + R;
+  float* row_f = row_l + R;
+  int64_t* k_at = reinterpret_cast<int64_t*>(smem + P::kOffKey);
+  int64_t* v_at = k_at + TK;
+  float* k_sc = reinterpret_cast<float*>(v_at + TK);
+  float* v_sc = k_sc + TK;
+  Cut* cut = reinterpret_cast<Cut*>(smem + P::kOffCut);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int d = a.c.d;
+
+  block_cut<256>(a, cut);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  Walk w;
+  w.init(a, cut);
+  while (w.next(a)) {
+    const int64_t rows_all = w.tokens * a.group;
+    const int rows = (int)(rows_all - w.row0 < R ? rows_all - w.row0 : R);
+    __syncthreads();
+    for (int x = tid; x < R * (DP / 4); x += 256) {
+      const int r = x / (DP / 4), e = (x % (DP / 4)) * 4;
+      float q[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r < rows) {
+        const int64_t xr = w.row0 + r, t = xr / a.group;
+        const TQ* src = reinterpret_cast<const TQ*>(a.Q) + (w.begin + t) * a.q_stride[0] +
+                        (w.h * (int64_t)a.group + (xr - t * a.group)) * a.q_stride[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (e + i < d) q[i] = up1(src[e + i]);
+      }
+      *reinterpret_cast<float4*>(Qs + r * PITCH + e) = make_float4(q[0], q[1], q[2], q[3]);
+    }
+    if (tid < R) {
+      row_m[tid] = neg_inf();
+      row_l[tid] = 0.f;
+    }
+    float o[4][P::NCG][4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int g = 0; g < P::NCG; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[r][g][i] = 0.f;
+    const int rg = tid & 3, cg = (tid >> 2) % P::CGT, ks = tid / (4 * P::CGT);
+
+    for (int64_t t = w.t0; t < w.t0 + w.n; ++t) {
+      __syncthreads();  // the last tile's K, V and P are done with
+      if (tid < TK) {
+        const int64_t p = t * TK + tid;
+        const int32_t page = p < w.len ? a.c.page_of(w.b, p) : -1;
+        k_at[tid] = -1;
+        if (page >= 0) {
+          const int32_t slot = a.c.slot_of(p);
+          k_at[tid] = a.c.K.at(page, slot, w.h);
+          v_at[tid] = a.c.V.at(page, slot, w.h);
+          if constexpr (IsByte<TC>::value) {
+            k_sc[tid] = a.c.K.scale[a.c.K.scale_at(page, slot, w.h)];
+            v_sc[tid] = a.c.V.scale[a.c.V.scale_at(page, slot, w.h)];
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int x = tid; x < TK * (DP / 4); x += 256) {
+        const int key = x / (DP / 4), e = (x % (DP / 4)) * 4;
+        float k[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+        const int64_t ka = k_at[key];
+        if (ka >= 0) {
+          const TC* kp = reinterpret_cast<const TC*>(a.c.K.data) + ka + e;
+          const TC* vp = reinterpret_cast<const TC*>(a.c.V.data) + v_at[key] + e;
+          if (vec) {  // d and every stride divide by 4
+            if (e < d) {
+              load_vec<TC, 4>(kp, k);
+              load_vec<TC, 4>(vp, v);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (e + i < d) {
+                k[i] = up1(kp[i]);
+                v[i] = up1(vp[i]);
+              }
+          }
+          if constexpr (IsByte<TC>::value) {
+            const float fk = k_sc[key], fv = v_sc[key];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              k[i] *= fk;
+              v[i] *= fv;
+            }
+          }
+        }
+        *reinterpret_cast<float4*>(Ks + key * PITCH + e) = make_float4(k[0], k[1], k[2], k[3]);
+        *reinterpret_cast<float4*>(Vs + key * PITCH + e) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+      __syncthreads();
+      {  // scores
+        const int kb = warp % P::KB, ds = warp / P::KB, r4 = lane >> 3, kg = lane & 7;
+        const float* qp = Qs + r4 * 4 * PITCH + ds * (DP / P::DS);
+        const float* kp = Ks + (kb * 16 + kg) * PITCH + ds * (DP / P::DS);
+        float s[4][2] = {};
+#pragma unroll 4
+        for (int e = 0; e < DP / P::DS; e += 4) {
+          const float4 k0 = *reinterpret_cast<const float4*>(kp + e);
+          const float4 k1 = *reinterpret_cast<const float4*>(kp + 8 * PITCH + e);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float4 q = *reinterpret_cast<const float4*>(qp + r * PITCH + e);
+            s[r][0] = fmaf(q.x, k0.x, fmaf(q.y, k0.y, fmaf(q.z, k0.z, fmaf(q.w, k0.w, s[r][0]))));
+            s[r][1] = fmaf(q.x, k1.x, fmaf(q.y, k1.y, fmaf(q.z, k1.z, fmaf(q.w, k1.w, s[r][1]))));
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          Ss[(ds * R + r4 * 4 + r) * TK + kb * 16 + kg] = s[r][0];
+          Ss[(ds * R + r4 * 4 + r) * TK + kb * 16 + kg + 8] = s[r][1];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int rr = 0; rr < 2; ++rr) {  // softmax: a warp takes two rows
+        constexpr int KL = (TK + 31) / 32;
+        const int r = warp * 2 + rr;
+        float s[KL], top = neg_inf();
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const int key = lane + 32 * i;
+          s[i] = neg_inf();
+          if (key < TK && k_at[key] >= 0) {
+            float x = 0.f;
+#pragma unroll
+            for (int ds = 0; ds < P::DS; ++ds) x += Ss[(ds * R + r) * TK + key];
+            s[i] = x * a.scale_log2e;
+          }
+          top = max_nan(top, s[i]);
+        }
+#pragma unroll
+        for (int o2 = 16; o2 > 0; o2 >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o2));
+        const float m_old = row_m[r], m_new = max_nan(m_old, top);
+        const float ref = m_new == neg_inf() ? 0.f : m_new;  // nothing seen yet: every exponent stays -inf
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const int key = lane + 32 * i;
+          const float p = fast_exp2(s[i] - ref);
+          sum += p;
+          if (key < TK) Ps[key * 20 + r] = p;
+        }
+#pragma unroll
+        for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o2);
+        __syncwarp();
+        if (lane == 0) {
+          const float f = fast_exp2(m_old - ref);
+          row_f[r] = f;
+          row_l[r] = row_l[r] * f + sum;
+          row_m[r] = m_new;
+        }
+      }
+      __syncthreads();
+      {  // O = O f + P V
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float f = row_f[rg * 4 + r];
+#pragma unroll
+          for (int g = 0; g < P::NCG; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][g][i] *= f;
+        }
+        constexpr int KPS = TK / P::KS;
+#pragma unroll 4
+        for (int key = ks * KPS; key < ks * KPS + KPS; ++key) {
+          const float4 p = *reinterpret_cast<const float4*>(Ps + key * 20 + rg * 4);
+#pragma unroll
+          for (int g = 0; g < P::NCG; ++g) {
+            const float4 v = *reinterpret_cast<const float4*>(Vs + key * PITCH + (g * P::CGT + cg) * 4);
+            const float pr[4] = {p.x, p.y, p.z, p.w}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[r][g][i] = fmaf(pr[r], vv[i], o[r][g][i]);
+          }
+        }
+      }
+    }
+    // the shares of the keys are added up where K and V were, then the rows leave
+    __syncthreads();
+    float* Os = Ks;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int g = 0; g < P::NCG; ++g)
+        *reinterpret_cast<float4*>(Os + (ks * R + rg * 4 + r) * DP + (g * P::CGT + cg) * 4) =
+            make_float4(o[r][g][0], o[r][g][1], o[r][g][2], o[r][g][3]);
+    __syncthreads();
+    const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0, blockIdx.x);
+    for (int x = tid; x < rows * (DP / 4); x += 256) {
+      const int r = x / (DP / 4), e = (x % (DP / 4)) * 4;
+      if (e >= a.d_pad) continue;
+      float4 y = *reinterpret_cast<const float4*>(Os + r * DP + e);
+#pragma unroll
+      for (int s2 = 1; s2 < P::KS; ++s2) {
+        const float4 z = *reinterpret_cast<const float4*>(Os + (s2 * R + r) * DP + e);
+        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+      }
+      *reinterpret_cast<float4*>(a.O + (out + r) * a.d_pad + e) = y;
+    }
+    if (tid < rows) a.ml[out + tid] = make_float2(row_m[tid], row_l[tid]);
+  }
+}
+
+// ---- merge kernel -----------------------------------------------------------------------------------------------------------
+//
+// One warp per row; a lane holds columns (i * 32 + lane) * VE. The drafted keys come first: they need nothing of the context
+// kernel, so their loads run while it drains. Four keys at a time keep eight row loads in flight.
+struct MergeArgs {
+  const uint8_t* mask;
+  int64_t mask_width;
+  float *m, *l;
+  char* O;
+  int64_t o_stride[2];
+  int first;
+};
+
+template <class TQ, class TC, int VE, int NC>
+__global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArgs g) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int64_t n = warp / a.n_q_heads;
+  const int32_t hq = (int32_t)(warp - n * a.n_q_heads);
+  const int32_t b = n < a.n_rows ? sequence_of(a.cu_rows, a.c.n_seq, n) : -1;
+  if (b < 0) return;
+  int64_t begin, end;
+  rows_of(a.cu_rows, b, a.n_rows, begin, end);
+  const int64_t tokens = end - begin, len = a.c.len_of(b);
+  const int32_t h = hq / a.group;
+  const int d = a.c.d;
+
+  float q[NC * VE], acc[NC * VE];
+  float M = neg_inf(), L = 0.f;
+  auto col = [&](int i) { return (i * 32 + lane) * VE; };
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    float x[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) x[e] = acc[i * VE + e] = 0.f;
+    if (col(i) < d) load_vec<TQ, VE>(reinterpret_cast<const TQ*>(a.Q) + n * a.q_stride[0] + hq * a.q_stride[1] + col(i), x);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) q[i * VE + e] = x[e];
+  }
+
+  constexpr int KB = NC * VE <= 8 ? 4 : 1;  // keys at a time: as registers allow
+  const int64_t cols = tokens < g.mask_width ? tokens : g.mask_width;
+  for (int64_t j0 = 0; j0 < cols; j0 += 32) {
+    const bool on = j0 + lane < cols && __ldg(g.mask + n * g.mask_width + j0 + lane) != 0;
+    // each lane finds the page of its own key, before the keys are taken one after the other
+    const int64_t p = len + j0 + lane;
+    const int32_t my_page = on ? a.c.page_of(b, p) : -1;
+    const int32_t my_slot = on ? a.c.slot_of(p) : 0;
+    unsigned bits = __ballot_sync(kFullMask, my_page >= 0);
+    while (bits) {
+      float k[KB][NC * VE], v[KB][NC * VE], s[KB], fv[KB];
+      int taken = 0;
+#pragma unroll
+      for (int x = 0; x < KB; ++x) {
+        s[x] = 0.f;
+        fv[x] = 1.f;
+#pragma unroll
+        for (int e = 0; e < NC * VE; ++e) k[x][e] = v[x][e] = 0.f;
+        if (bits == 0) continue;
+        const int j = __ffs(bits) - 1;
+        bits &= bits - 1;
+        ++taken;
+        const int32_t page = __shfl_sync(kFullMask, my_page, j), slot = __shfl_sync(kFullMask, my_slot, j);
+        const TC* kp = reinterpret_cast<const TC*>(a.c.K.data) + a.c.K.at(page, slot, h);
+        const TC* vp = reinterpret_cast<const TC*>(a.c.V.data) + a.c.V.at(page, slot, h);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (col(i) < d) {
+            float y[VE];
+            load_vec<TC, VE>(kp + col(i), y);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) k[x][i * VE + e] = y[e];
+            load_vec<TC, VE>(vp + col(i), y);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) v[x][i * VE + e] = y[e];
+          }
+        if constexpr (IsByte<TC>::value) {
+          s[x] = a.c.K.scale[a.c.K.scale_at(page, slot, h)];
+          fv[x] = a.c.V.scale[a.c.V.scale_at(page, slot, h)];
+        } else {
+          s[x] = 1.f;
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int x = 0; x < KB; ++x) {
+        float y = 0.f;
+#pragma unroll
+        for (int e = 0; e < NC * VE; ++e) y = fmaf(q[e], IsByte<TC>::value ? k[x][e] * s[x] : k[x][e], y);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(kFullMask, y, o);
+        s[x] = x < taken ? y * a.scale_log2e : neg_inf();
+        top = max_nan(top, s[x]);
+      }
+      const float ref = top == neg_inf() ? 0.f : top;
+      const float f = fast_exp2(M - ref);
+      L *= f;
+#pragma unroll
+      for (int e = 0; e < NC * VE; ++e) acc[e] *= f;
+#pragma unroll
+      for (int x = 0; x < KB; ++x) {
+        if (x >= taken) continue;
+        const float pr = fast_exp2(s[x] - ref);
+        L += pr;
+#pragma unroll
+        for (int e = 0; e < NC * VE; ++e) acc[e] = fmaf(pr, IsByte<TC>::value ? v[x][e] * fv[x] : v[x][e], acc[e]);
+      }
+      M = top;
+    }
+  }
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t tiles = a.tiles_of(len);
+  if (tiles > 0) {
+    const int64_t x = (n - begin) * a.group + (hq - (int64_t)h * a.group);
+    const int64_t u = (int64_t)h * a.row_tiles(tokens) + x / a.row_tile;
+    const int64_t chunk = a.cut[0], t = a.cut[1 + b] + u * tiles;
+    const int64_t c0 = t / chunk, c1 = (t + tiles - 1) / chunk;
+    for (int64_t c = c0; c <= c1; c += 32) {
+      const int np = (int)(c1 - c + 1 < 32 ? c1 - c + 1 : 32);
+      const int64_t row = a.partial_row(begin, tokens, h, x, c);
+      float2 ml = make_float2(neg_inf(), 0.f);
+      if (lane < np) ml = a.ml[row + (int64_t)lane * a.row_tile];
+      float top = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o));
+      top = max_nan(top, M);
+      const float ref = top == neg_inf() ? 0.f : top;
+      const float f = fast_exp2(M - ref), wgt = fast_exp2(ml.x - ref);
+      float sum = wgt * ml.y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+      L = L * f + sum;
+#pragma unroll
+      for (int e = 0; e < NC * VE; ++e) acc[e] *= f;
+#pragma unroll 4
+      for (int k = 0; k < np; ++k) {
+        const float wk = __shfl_sync(kFullMask, wgt, k);
+        const float* src = a.O + (row + (int64_t)k * a.row_tile) * a.d_pad;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (col(i) < d) {
+            float y[VE];
+            load_vec<float, VE>(src + col(i), y);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[i * VE + e] = fmaf(wk, y[e], acc[i * VE + e]);
+          }
+      }
+      M = top;
+    }
+  }
+
+  float* m = g.m + n * a.n_q_heads + hq;
+  float* l = g.l + n * a.n_q_heads + hq;
+  const bool none = M == neg_inf();  // no key, or none with a score above -inf
+  if (none && !g.first) return;
+  TQ* O = reinterpret_cast<TQ*>(g.O) + n * g.o_stride[0] + hq * g.o_stride[1];
+  float m_out = M * 0.6931471805599453f, keep = 0.f, mine = 1.f;
+  if (!g.first) {
+    const float m_in = *m, l_in = *l;
+    if (l_in != 0.f) {  // a row with l = 0 is empty: what its O holds does not count
+      const float m2 = m_in * kLog2e, top = max_nan(m2, M);
+      if (!(M > m2)) m_out = top != top ? top : m_in;
+      mine = fast_exp2(M - top);
+      keep = l_in * fast_exp2(m2 - top);
+      L = fmaf(L, mine, keep);
+    }
+  }
+  const float inv = none ? 0.f : 1.f / L;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (col(i) < d) {
+      float y[VE];
+      if (keep != 0.f) load_vec<TQ, VE>(O + col(i), y);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float x = acc[i * VE + e] * mine;
+        y[e] = (keep != 0.f ? fmaf(keep, y[e], x) : x) * inv;
+      }
+      store_vec<TQ, VE>(O + col(i), y);
+    }
+  __syncwarp();
+  if (lane == 0) {
+    *m = m_out;
+    *l = none ? 0.f : L;
+  }
+}
+
+}  // namespace tree
+}  // namespace spfa

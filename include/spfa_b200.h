@@ -374,6 +374,68 @@ int spfa_global_no_local_forward_16(int dtype, const void* Q, const void* K, con
                                     int64_t local_size_each_dir, int64_t row_begin, int64_t row_end,
                                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- paged key / value caches, and attention of drafted token trees over them --------------------------------------------
+ * No counterpart in the reference (its K and V are dense matrices of one head).
+ *
+ * A cache holds K and V of every key head in pages of page_size positions. Position p of sequence b lies in page
+ * page_table[b * table_width + p / page_size], slot p % page_size; lens[b] positions of it are committed. Element [page][slot]
+ * [head][0 .. d) of K starts K_stride[0] * page + K_stride[1] * slot + K_stride[2] * head elements behind K; both orders of
+ * slots and heads, slices of larger tensors, and K and V interleaved in one allocation are such strides. dtype is what the
+ * pages hold:
+ *   SPFA_DTYPE_F32, _F16, _BF16   the values themselves (calls then take rows of the same type)
+ *   SPFA_DTYPE_E4M3               8-bit floating point times the row's scale 2^e, e >= -126 the smallest with max|x| <= 448 2^e
+ *   SPFA_DTYPE_INT8               rn(x * (127 / max|x|)) with the row's scale max|x| / 127, both quotients rounded to float32;
+ *                                 rows with max|x| < 2^-100 are held as zeros
+ * A row is one head of one position; its scale is K_scale[K_scale_stride . (page, slot, head)]. A row with a value that is
+ * not finite is held with scale NaN: it reads back as NaN, and rows that attend to it become NaN.
+ * The struct lives in host memory and is read during the call; everything it points to is device memory.
+ *
+ * Calls on rows take cu_rows[n_seq + 1] (device, ascending): row i belongs to the sequence b with cu_rows[b] <= i < cu_rows[b + 1]
+ * and stands for position lens[b] + i - cu_rows[b]. Rows that belong to no sequence are left as they are, and so are rows whose
+ * position does not exist: a position at or behind table_width * page_size, from 2^31 - 1 on, or in a page whose number is not in
+ * [0, n_pages), is neither read nor written, and nobody attends to it. Lengths below 0 count as 0 where keys are counted.
+ * Sequences may share pages; a call that writes one position twice leaves either of the two there. */
+enum { SPFA_DTYPE_E4M3 = 3, SPFA_DTYPE_INT8 = 4 };
+typedef struct spfa_kv_cache {
+  void *K, *V;
+  float *K_scale, *V_scale;            /* only of the 8-bit types, else ignored */
+  int64_t K_stride[3], V_stride[3];    /* elements from page to page, slot to slot, head to head */
+  int64_t K_scale_stride[3], V_scale_stride[3];
+  int64_t n_pages, page_size, n_heads;
+  const int32_t* page_table;           /* [n_seq][table_width] */
+  const int32_t* lens;                 /* [n_seq] */
+  int64_t n_seq, table_width;
+  int32_t d, dtype;
+} spfa_kv_cache;
+
+/* Rows K[i * K_stride[0] + h * K_stride[1] + 0 .. d) and V are written to their positions in the cache, in its type. */
+int spfa_cache_append(const spfa_kv_cache* cache, int dtype, const void* K, const int64_t* K_stride, const void* V,
+                      const int64_t* V_stride, const int32_t* cu_rows, int64_t n_rows, void* stream);
+/* The way back: rows K and V of type dtype are filled from the cache (q * scale in float32, rounded once). */
+int spfa_cache_read(const spfa_kv_cache* cache, int dtype, void* K, const int64_t* K_stride, void* V, const int64_t* V_stride,
+                    const int32_t* cu_rows, int64_t n_rows, void* stream);
+/* Position lens[b] + i := position lens[b] + kept[b * width + i], for i < n_kept[b] (at most width). kept[b] is ascending without
+ * repeats: the drafted tokens on the accepted path. Rows are moved as they are held, scales included. */
+int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t width, const int32_t* n_kept, void* stream);
+
+/* Attention of drafted rows: query row i of sequence b, head hq, attends with key head hq / (n_q_heads / n_heads) to
+ *   every committed position [0, lens[b])   and   the drafted positions lens[b] + j with tree_mask[i * mask_width + j] != 0
+ * (j below the sequence's number of rows and below mask_width), whose K and V the cache already holds. Scores, (m, l, O) and
+ * their update are those of the other operators; m and l are float32 [n_rows, n_q_heads], contiguous, whatever the type of Q
+ * and O is. With first != 0 the incoming state is taken as empty and not read, and every row of a sequence is written: rows that
+ * see no key get m = -inf, l = 0, O = 0. With first = 0 such rows are left as they are, and an incoming row with l = 0 is empty:
+ * its O does not count. O may be Q itself (same strides); otherwise nothing that is written may overlap anything that is read.
+ *
+ * dtype: type of Q and O (equal to the cache's where that holds its values as they are). float32 calls compute in float32.
+ * 16-bit calls run the committed positions on the tensor cores where d is at most 128, rows are 16-byte aligned (d a multiple
+ * of 8, of an 8-bit cache 16) and pages hold a multiple of 8 positions or at least 64; their probabilities enter the product with
+ * V as one 16-bit number each (bfloat16 where the cache is 8-bit or bfloat16). Everything else is computed in float32.
+ * The workspace needs spfa_tree_workspace_bytes of the same cache, n_rows and n_q_heads. */
+size_t spfa_tree_workspace_bytes(const spfa_kv_cache* cache, int dtype, int64_t n_rows, int64_t n_q_heads);
+int spfa_tree_forward(const spfa_kv_cache* cache, int dtype, const void* Q, const int64_t* Q_stride, const int32_t* cu_rows,
+                      int64_t n_rows, int64_t n_q_heads, const uint8_t* tree_mask, int64_t mask_width, float* m, float* l, void* O,
+                      const int64_t* O_stride, int first, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- dense boolean mask -> CSR / COO arrays on the GPU ----------------------------------------------------
  * No counterpart in the reference: its callers convert a dense [n_rows, n_cols] boolean mask with torch's
  * to_sparse_csr() / to_sparse_coo() and cast the index tensors (verification/verify.py:67-71, 94-98). These two
