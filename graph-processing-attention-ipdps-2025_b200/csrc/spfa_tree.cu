@@ -9,13 +9,14 @@ namespace {
 constexpr int kCtas = 296;  // of the context kernel: two on each of 148 SMs
 
 struct TreeLayout {
-  int row_tile, d_pad;
+  int row_tile, d_pad;  // row_tile: of the larger units
   int64_t rows;
   size_t cut, ml, O, total;
 };
-TreeLayout tree_layout(const spfa_kv_cache* c, int64_t n_rows, int64_t n_q_heads) {
+TreeLayout tree_layout(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
   TreeLayout t{};
-  t.row_tile = tree::kAnyRows;
+  // either context kernel must fit: which one runs is settled by the call
+  t.row_tile = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? tree::kTiledRows : tree::kAnyRows;
   t.d_pad = (c->d + 3) / 4 * 4;
   t.rows = n_rows * n_q_heads + (int64_t)t.row_tile * kCtas;
   t.cut = 0;
@@ -33,6 +34,18 @@ int check_tree(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_he
   return SPFA_OK;
 }
 
+bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride) {
+  if (dtype == SPFA_DTYPE_F32 || !tree::tiled_shape(c) || !rows_align(Q, Q_stride, 2, 8)) return false;
+  return dtype == SPFA_DTYPE_F16 ? tree::usable_f16(c) : tree::usable_bf16(c);
+}
+
+// One wave of CTAs, or as many as there can be shares of the list: lens is not known here, the page lists bound it.
+int grid_of(const tree::Call& a) {
+  const double tiles = (double)a.tiles_of(a.c.capacity), rows = (double)a.n_rows * a.group / a.row_tile + a.c.n_seq;
+  const double most = tiles * rows * a.c.n_heads / a.least;
+  return most < kCtas ? (most < 1 ? 1 : (int)most) : kCtas;
+}
+
 }  // namespace
 }  // namespace spfa
 
@@ -41,7 +54,7 @@ using namespace spfa;
 extern "C" {
 
 size_t spfa_tree_workspace_bytes(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
-  return check_tree(c, dtype, n_rows, n_q_heads) == SPFA_OK ? tree_layout(c, n_rows, n_q_heads).total : 0;
+  return check_tree(c, dtype, n_rows, n_q_heads) == SPFA_OK ? tree_layout(c, dtype, n_rows, n_q_heads).total : 0;
 }
 
 int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride, const int32_t* cu_rows,
@@ -53,7 +66,7 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   if (!Q || !Q_stride || !cu_rows || !m || !l || !O || !O_stride || mask_width < 0 || (mask_width > 0 && !tree_mask)) return SPFA_ERR_BAD_ARG;
   if (!aligned_to(Q, size) || !aligned_to(O, size) || !aligned4(cu_rows) || !aligned4(m) || !aligned4(l)) return SPFA_ERR_BAD_ARG;
   if (Q_stride[0] < 0 || Q_stride[1] < 0 || O_stride[0] < 0 || O_stride[1] < 0) return SPFA_ERR_BAD_ARG;
-  const TreeLayout t = tree_layout(c, n_rows, n_q_heads);
+  const TreeLayout t = tree_layout(c, dtype, n_rows, n_q_heads);
   rc = check_workspace(workspace, workspace_bytes, t.total);
   if (rc != SPFA_OK) return rc;
   if (n_rows == 0 || c->n_seq == 0) return SPFA_OK;
@@ -68,11 +81,20 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   a.n_q_heads = (int32_t)n_q_heads;
   a.group = (int32_t)(n_q_heads / c->n_heads);
   a.scale_log2e = (1.0f / sqrtf((float)c->d)) * kLog2e;
-  a.row_tile = t.row_tile;
-  a.tile_keys = tree::any_tile_keys(c->d);
-  a.page_tiles = 0;
+  const bool tiled = g_path.load() != SPFA_PATH_GATHER && tiled_call(c, dtype, Q, Q_stride);
+  if (g_path.load() == SPFA_PATH_TILED && !tiled) return SPFA_ERR_BAD_ARG;
+  if (tiled) {
+    a.row_tile = tree::kTiledRows;
+    const int ps = a.c.page_size, keys = tree::kTiledKeys;
+    a.page_tiles = ps >= keys ? (ps + keys - 1) / keys : 0;
+    a.tile_keys = ps >= keys ? keys : keys / ps * ps;
+  } else {
+    a.row_tile = tree::kAnyRows;
+    a.tile_keys = tree::any_tile_keys(c->d);
+    a.page_tiles = 0;
+  }
   a.least = 1;
-  a.n_cta = kCtas;
+  a.n_cta = grid_of(a);
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
   a.ml = reinterpret_cast<float2*>(ws + t.ml);
@@ -89,9 +111,9 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   g.first = first ? 1 : 0;
   const bool vec = cache_rows_align(c, 4) && rows_align(Q, Q_stride, size, 4) && rows_align(O, O_stride, size, 4);
   cudaStream_t st = (cudaStream_t)stream;
-  g_last_path.store(SPFA_PATH_GATHER);
-  if (dtype == SPFA_DTYPE_F16) return tree::launch_f16(c, a, g, vec, st);
-  if (dtype == SPFA_DTYPE_BF16) return tree::launch_bf16(c, a, g, vec, st);
+  g_last_path.store(tiled ? SPFA_PATH_TILED : SPFA_PATH_GATHER);
+  if (dtype == SPFA_DTYPE_F16) return tree::launch_f16(c, a, g, vec, tiled, st);
+  if (dtype == SPFA_DTYPE_BF16) return tree::launch_bf16(c, a, g, vec, tiled, st);
   return tree::launch_f32(c, a, g, vec, st);
 }
 

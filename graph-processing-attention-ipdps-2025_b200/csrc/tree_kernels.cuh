@@ -43,7 +43,7 @@ struct Call {
   float* O;       // [rows][d_pad]
   int32_t d_pad;
 
-  __device__ __forceinline__ int64_t tiles_of(int64_t len) const {
+  __host__ __device__ __forceinline__ int64_t tiles_of(int64_t len) const {
     if (page_tiles == 0) return (len + tile_keys - 1) / tile_keys;
     const int64_t full = len / c.page_size, rest = len - full * c.page_size;
     return full * page_tiles + (rest + tile_keys - 1) / tile_keys;
@@ -126,19 +126,21 @@ __device__ __forceinline__ void block_cut(const Call& a, Cut* s) {
   }
 }
 
-// Walks the pieces of a CTA: piece = consecutive key tiles [t0, t0 + n) of one unit. Every role of a CTA walks on its own.
+// Walks the pieces of a CTA: piece = consecutive key tiles [t0, t0 + n) of one unit. Every role of a CTA walks on its own. Rows, key
+// tiles of a sequence and positions fit in 32 bits, the list does not have to.
 struct Walk {
-  int64_t at, last, start, weight, begin, tokens, len, tiles;
-  int32_t b, h;
-  int64_t row0;  // first row of the unit's row tile among the tokens * group rows of the key head
-  int64_t t0, n;
+  int64_t at, last, start, weight;
+  int32_t b, h, begin, tokens, len, tiles;
+  int32_t row0;  // first row of the unit's row tile among the tokens * group rows of the key head
+  int32_t t0, n;
 
   __device__ __forceinline__ void open(const Call& a) {
-    int64_t end;
-    rows_of(a.cu_rows, b, a.n_rows, begin, end);
-    tokens = end - begin;
-    len = a.c.len_of(b);
-    tiles = a.tiles_of(len);
+    int64_t x, y;
+    rows_of(a.cu_rows, b, a.n_rows, x, y);
+    begin = (int32_t)x;
+    tokens = (int32_t)(y - x);
+    len = (int32_t)a.c.len_of(b);
+    tiles = (int32_t)a.tiles_of(len);
     weight = tokens ? tiles * a.row_tiles(tokens) * a.c.n_heads : 0;
   }
   __device__ __forceinline__ void init(const Call& a, const Cut* s) {
@@ -158,13 +160,18 @@ struct Walk {
       ++b;
       open(a);
     }
-    const int64_t u = (at - start) / tiles;
-    t0 = (at - start) - u * tiles;
-    n = tiles - t0 < last - at ? tiles - t0 : last - at;
-    const int64_t rt = a.row_tiles(tokens);
+    const uint64_t in = (uint64_t)(at - start);
+    const uint32_t u = (uint32_t)(in / (uint32_t)tiles);
+    t0 = (int32_t)(in - (uint64_t)u * (uint32_t)tiles);
+    n = tiles - t0 < last - at ? tiles - t0 : (int32_t)(last - at);
+    const uint32_t rt = (uint32_t)a.row_tiles(tokens);
     h = (int32_t)(u / rt);
-    row0 = (u - (int64_t)h * rt) * a.row_tile;
+    row0 = (int32_t)(u - (uint32_t)h * rt) * a.row_tile;
     return true;
+  }
+  __device__ __forceinline__ int rows(const Call& a) const {  // of the unit
+    const int32_t left = tokens * a.group - row0;
+    return left < a.row_tile ? left : a.row_tile;
   }
 };
 
@@ -212,15 +219,14 @@ __global__ void __launch_bounds__(256) context_any_kernel(const Call a, const in
   Walk w;
   w.init(a, cut);
   while (w.next(a)) {
-    const int64_t rows_all = w.tokens * a.group;
-    const int rows = (int)(rows_all - w.row0 < R ? rows_all - w.row0 : R);
+    const int rows = w.rows(a);
     __syncthreads();
     for (int x = tid; x < R * (DP / 4); x += 256) {
       const int r = x / (DP / 4), e = (x % (DP / 4)) * 4;
       float q[4] = {0.f, 0.f, 0.f, 0.f};
       if (r < rows) {
-        const int64_t xr = w.row0 + r, t = xr / a.group;
-        const TQ* src = reinterpret_cast<const TQ*>(a.Q) + (w.begin + t) * a.q_stride[0] +
+        const int32_t xr = w.row0 + r, t = xr / a.group;
+        const TQ* src = reinterpret_cast<const TQ*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
                         (w.h * (int64_t)a.group + (xr - t * a.group)) * a.q_stride[1];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -241,10 +247,10 @@ __global__ void __launch_bounds__(256) context_any_kernel(const Call a, const in
         for (int i = 0; i < 4; ++i) o[r][g][i] = 0.f;
     const int rg = tid & 3, cg = (tid >> 2) % P::CGT, ks = tid / (4 * P::CGT);
 
-    for (int64_t t = w.t0; t < w.t0 + w.n; ++t) {
+    for (int32_t t = w.t0; t < w.t0 + w.n; ++t) {
       __syncthreads();  // the last tile's K, V and P are done with
       if (tid < TK) {
-        const int64_t p = t * TK + tid;
+        const int64_t p = (int64_t)t * TK + tid;
         const int32_t page = p < w.len ? a.c.page_of(w.b, p) : -1;
         k_at[tid] = -1;
         if (page >= 0) {

@@ -1,15 +1,22 @@
 // Host side of the tree attention, one translation unit per type of Q: the kernels are compiled in parallel.
 #pragma once
 #include "cache_view.cuh"
+#include "tensor_map.cuh"
 #include "tree_kernels.cuh"
+#include "tree_tiled.cuh"
 
 namespace spfa {
 namespace tree {
 
-// Launches the context and merge kernels of one call; `vec`: rows of Q, O and the cache are whole 4-element pieces.
+// Launches the context and merge kernels of one call. `vec`: rows of Q, O and the cache are whole 4-element pieces; `tiled`: on the
+// tensor cores (16-bit only; the caller has checked tiled_shape). The *_usable functions: whether this build's kernels can run.
 int launch_f32(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st);
-int launch_f16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st);
-int launch_bf16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st);
+int launch_f16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, bool tiled, cudaStream_t st);
+int launch_bf16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, bool tiled, cudaStream_t st);
+bool usable_f16(const spfa_kv_cache* c);
+bool usable_bf16(const spfa_kv_cache* c);
+
+constexpr int kTiledRows = 128, kTiledKeys = 64;  // unit and tile of context_tiled_kernel
 
 constexpr int kAnyRows = 16;  // row tile of context_any_kernel
 inline int any_tile_keys(int d) { return d <= 128 ? 64 : (d <= 256 ? 32 : 16); }
@@ -76,6 +83,90 @@ int launch_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
   else if (d <= 512) rc = launch_context_any<512, TQ, TC>(a, vec, st);
   else rc = launch_context_any<1024, TQ, TC>(a, vec, st);
   return rc != SPFA_OK ? rc : launch_merge_any<TQ, TC>(a, g, vec, st);
+}
+
+// What the copy engine can address: 16-byte rows and strides below 2^40 bytes, boxes that do not cut a page into unaligned pieces.
+inline bool tiled_shape(const spfa_kv_cache* c) {
+  const int size = dtype_bytes(c->dtype);
+  if (c->d > 128 || c->n_pages < 1 || !cache_rows_align(c, 16 / size) || (c->page_size % 8 && c->page_size < kTiledKeys)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (c->K_stride[i] * size >= (1LL << 40) || c->V_stride[i] * size >= (1LL << 40)) return false;
+  return true;
+}
+
+// Pages as (element, slot, head, page), fetched as boxes of a page's slots (at most kTiledKeys) x 128 bytes of 16-bit elements in the
+// swizzle of the tensor cores, or x `dp` codes of an 8-bit cache as they lie. Elements behind d and slots behind a page are zeros.
+template <class T>
+bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const int64_t* stride, int dp) {
+  TensorMapEncodeTiledFn enc = tensor_map_encoder();
+  if (!enc) return false;
+  constexpr bool kByte = sizeof(T) == 1;
+  const cuuint64_t dims[4] = {(cuuint64_t)c->d, (cuuint64_t)c->page_size, (cuuint64_t)c->n_heads, (cuuint64_t)c->n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)stride[1] * sizeof(T), (cuuint64_t)stride[2] * sizeof(T), (cuuint64_t)stride[0] * sizeof(T)};
+  for (int i = 0; i < 3; ++i)
+    if (strides[i] == 0) strides[i] = 16;  // of a dimension of one element
+  const cuuint32_t box[4] = {kByte ? (cuuint32_t)dp : 64u, (cuuint32_t)(c->page_size < kTiledKeys ? c->page_size : kTiledKeys), 1u, 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUtensorMapDataType type = kByte ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                         : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+  return enc(tm, type, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             kByte ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// As band16_usable: setmaxnreg.inc must be covered by what the launch allocates.
+template <int DP, class T, class TC>
+bool tiled_usable() {
+  using P = PlanTree<DP, TC>;
+  static std::atomic<int> cached[64];  // per device: 0 unknown, 1 usable, 2 not
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  int v = cached[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    cudaFuncAttributes attr;
+    auto kern = context_tiled_kernel<DP, T, TC>;
+    const bool ok = cudaFuncGetAttributes(&attr, kern) == cudaSuccess &&
+                    attr.numRegs * P::kThreads >= P::kRegsNeeded &&
+                    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kDynSmem) == cudaSuccess;
+    v = ok ? 1 : 2;
+    cached[dev].store(v, std::memory_order_relaxed);
+  }
+  return v == 1;
+}
+
+// f(tag of the cache's type, padded d)
+template <class TQ, class F>
+auto with_tiled(const spfa_kv_cache* c, F&& f) {
+  auto by_d = [&](auto* t) {
+    return c->d <= 64 ? f(t, std::integral_constant<int, 64>()) : f(t, std::integral_constant<int, 128>());
+  };
+  if (c->dtype == SPFA_DTYPE_E4M3) return by_d(static_cast<e4m3*>(nullptr));
+  if (c->dtype == SPFA_DTYPE_INT8) return by_d(static_cast<int8_t*>(nullptr));
+  return by_d(static_cast<TQ*>(nullptr));
+}
+
+template <class TQ>
+bool usable_by_cache(const spfa_kv_cache* c) {
+  return with_tiled<TQ>(c, [](auto* t, auto dp) {
+    return tiled_usable<decltype(dp)::value, TQ, typename std::remove_pointer<decltype(t)>::type>();
+  });
+}
+
+template <class TQ>
+int launch_tiled(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
+  return with_tiled<TQ>(c, [&](auto* t, auto dp) -> int {
+    using TC = typename std::remove_pointer<decltype(t)>::type;
+    constexpr int DP = decltype(dp)::value;
+    using P = PlanTree<DP, TC>;
+    int* err = tile_error_word();
+    CUtensorMap tmK, tmV;
+    if (!err || !make_page_map<TC>(&tmK, c, c->K, c->K_stride, DP) || !make_page_map<TC>(&tmV, c, c->V, c->V_stride, DP))
+      return SPFA_ERR_LAUNCH;
+    context_tiled_kernel<DP, TQ, TC><<<(unsigned)a.n_cta, P::kThreads, P::kDynSmem, st>>>(tmK, tmV, a, err);
+    g_launches.fetch_add(1);
+    const int rc = launch_status();
+    return rc != SPFA_OK ? rc : launch_merge_any<TQ, TC>(a, g, vec, st);
+  });
 }
 
 template <class TQ>

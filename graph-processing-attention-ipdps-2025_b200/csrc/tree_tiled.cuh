@@ -1,0 +1,673 @@
+// Tree attention over the committed positions on the tensor cores: float16 / bfloat16 Q, a cache of the same type or of 8 bits,
+// d <= 128. Part of the scheme of tree_kernels.cuh (units, pieces, partial rows).
+//
+// One CTA, two on an SM, takes its share of the list of key tiles piece by piece. A unit is 128 query rows (tokens x the query
+// heads of one key head) and a tile 64 keys:
+//   S  = Q K_j^T           128 x 64 fp32 in TMEM, two buffers, issued two tiles ahead
+//   P  = exp2(S c - shift) in registers, one thread a row, rounded to 16 bits and written over S
+//   O += P V_j             128 x DP fp32 in TMEM
+// Rows beyond a unit's are not computed: their warps only keep step. Roles (256 threads):
+//   warps 0-3  softmax and the pieces' epilogue: thread t <-> row t <-> TMEM lane t
+//   warp 4     TMA producer of K, masks and scales: page numbers 32 at a time in the lanes, one box for each page of a tile and 128
+//              bytes of d. Pages that do not exist are fetched from behind the last one, where the copy engine fills with zeros.
+//   warp 5     MMA issuer
+//   warp 6     TMA producer of V
+//   warp 7     Q
+//   warps 8-11 (8-bit caches) the conversion of each tile to 16 bits, and Q instead of warp 7
+// An 8-bit tile meets the tensor cores as float16 numbers that equal its codes (11 bits hold e4m3 and int8). The rows' scales stay in
+// fp32: K's multiplies the score, V's the probability before that is rounded, relative to the largest of the scales so far (a power
+// of two that the accumulator gives up when it grows). bfloat16 Q rows become float16 times a power of two: none of their 8 bits is
+// lost above 2^-29 of the row's largest element, and below nothing that a float32 sum of the products would show.
+// P is rounded to 16 bits. Where that alone would be as large as the rounding of the result (all but 8-bit caches under bfloat16 Q),
+// units of a single row tile carry a second 16-bit term, the rounding's remainder: they wait for memory, and the second product is
+// hidden. Units with more row tiles are bound by arithmetic and rows enough that the error stays at its mean, sqrt(2) of the
+// result's own rounding.
+#pragma once
+#include "tile_kernels_16.cuh"
+#include "tree_kernels.cuh"
+
+namespace spfa {
+namespace tree {
+
+using namespace tile;
+
+template <int DP, class TC>
+struct PlanTree {
+  static constexpr bool kQuant = sizeof(TC) == 1;
+  static constexpr int kThreads = kQuant ? 384 : 256, kRegsLaunch = kQuant ? 80 : 128;
+  static constexpr int kRegsSoftmax = kQuant ? 128 : 168, kRegsAux = kQuant ? 56 : 88, kQThreads = kQuant ? 128 : 32;
+  static constexpr int kRegsNeeded = kRegsSoftmax * 128 + kRegsAux * (kThreads - 128);
+  static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
+  static constexpr int TK = 64, kRows = 128, kChunks = DP / 64;
+  static constexpr int kQChunk = kRows * 128, kKVChunk = TK * 128, kQBytes = kChunks * kQChunk;
+  static constexpr int kTile = kChunks * kKVChunk;               // a 16-bit tile of K or V
+  static constexpr int kStage = kQuant ? TK * DP : kTile;        // a tile as it is fetched
+  static constexpr int NS = DP == 128 ? 2 : 4;                   // stages of K and of V
+  static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
+  static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStage, kOffCK = kOffV + NS * kStage;
+  static constexpr int kOffCV = kOffCK + (kQuant ? kTile : 0), kOffScale = kOffCV + (kQuant ? kTile : 0);
+  static constexpr int kOffQInv = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffQInv + (kQuant ? 2 * kRows * 4 : 0);
+  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 2 + 4 * NS + 4 + 6;
+  static constexpr int kOffCut = kOffBar + kNumBars * 8, kOffMisc = kOffCut + (int)sizeof(Cut);
+  static constexpr int kDynSmem = kOffMisc + 16 + 1024;
+  static_assert(2 * (kDynSmem + 1024) <= 228 * 1024, "two CTAs share an SM");
+  // The producer writes the ring's entry of a tile once the tile NS before has left its stage, which is behind the softmax of the
+  // tile two (8-bit: three) before that one.
+  static_assert(NS + 3 <= kRing, "ring entries are written again only after they were read");
+  static constexpr int kColS = 0, kColO = 2 * TK, kTmemCols = 256;
+  static_assert(kColO + DP <= kTmemCols, "S buffers and the O accumulator exceed the TMEM allocation");
+  static __device__ __forceinline__ uint32_t unit(int row, int u) { return (uint32_t)(row * 128 + ((u ^ (row & 7)) << 4)); }
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm, int32_t x, int32_t y, int32_t z, int32_t w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// Four codes to float16. The bytes of an int8 word leave in the order 0 2 1 3, where masks alone widen them: the order of d does not
+// matter to Q K^T as long as Q has it too, and O's columns are put right when they are stored.
+template <class TC> struct Widen {  // a cache that holds its values as they are is not converted
+  static constexpr bool kSwap = false;
+};
+template <> struct Widen<e4m3> {
+  static constexpr bool kSwap = false;
+  static __device__ __forceinline__ void four(uint32_t w, uint32_t& a, uint32_t& b) {
+    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    a = (uint32_t)x.x | ((uint32_t)x.y << 16);
+    b = (uint32_t)y.x | ((uint32_t)y.y << 16);
+  }
+};
+template <> struct Widen<int8_t> {
+  static constexpr bool kSwap = true;
+  // 1024 + (code + 128) has the code's bits as its last, and 1152 less is exact
+  static __device__ __forceinline__ uint32_t off(uint32_t x) {
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2(__half2_raw{0x6480, 0x6480}));
+    return *reinterpret_cast<const uint32_t*>(&y);
+  }
+  static __device__ __forceinline__ void four(uint32_t w, uint32_t& a, uint32_t& b) {
+    a = off((w & 0x00ff00ffu) ^ 0x64806480u);
+    b = off(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u);
+  }
+};
+
+// p V_j for an infinite V_j is that infinity, but the products of p's two terms need not add up to it: a term that is zero or negative
+// makes NaN. Where a piece's accumulator is not finite, V itself tells what it has to hold: +inf, -inf, or NaN where both or a NaN are
+// among the keys [p, p_end) that all rows of the piece see. Column `col` of one lane; returned: -1, 1, 2 (NaN) or 0 (all finite).
+template <class T>
+__device__ __noinline__ int infinity_of(const Call& a, int32_t b, int32_t h, int32_t p, int32_t p_end, int col) {
+  const float inf = __int_as_float(0x7f800000);
+  bool up = false, down = false, nan = false;
+  for (; p < p_end; ++p) {
+    const int32_t page = a.c.page_of(b, p);
+    if (page < 0 || col >= a.c.d) continue;
+    const float x = Half16<T>::up1(reinterpret_cast<const T*>(a.c.V.data)[a.c.V.at(page, a.c.slot_of(p), h) + col]);
+    up |= x == inf;
+    down |= x == -inf;
+    nan |= x != x;
+  }
+  return (nan || (up && down)) ? 2 : up ? 1 : down ? -1 : 0;
+}
+
+template <int DP, class T, class TC>
+__global__ void __launch_bounds__(PlanTree<DP, TC>::kThreads, 2)
+context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Call a,
+                     int* __restrict__ err) {
+  using P = PlanTree<DP, TC>;
+  constexpr int TK = P::TK, NS = P::NS;
+  constexpr bool kQuant = P::kQuant;
+  using TP = typename std::conditional<kQuant, __half, T>::type;  // operands of both products
+  constexpr bool kMaySplit = !(kQuant && std::is_same<T, __nv_bfloat16>::value);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + P::kOffBar + 8u * i; };
+  constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = 2 + NS, B_VFULL = 2 + 2 * NS, B_VEMPTY = 2 + 3 * NS,
+                B_CK = 2 + 4 * NS /* full, empty */, B_CV = B_CK + 2, B_SREADY = B_CK + 4, B_PREADY = B_SREADY + 2, B_OREADY = B_SREADY + 4;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::kOffMisc + 4);
+  Cut* cut = reinterpret_cast<Cut*>(smem + P::kOffCut);
+  uint64_t* ring_mask = reinterpret_cast<uint64_t*>(smem + P::kOffMask);
+  float* ring_scale = reinterpret_cast<float*>(smem + P::kOffScale);  // [ring][K, V][TK]
+  float* q_inv = reinterpret_cast<float*>(smem + P::kOffQInv);        // [unit parity][row]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t ps = a.c.page_size;
+  const int n_pages_tile = a.page_tiles ? 1 : a.tile_keys / ps;  // pages of a tile
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(B_QFULL), P::kQThreads);
+    mbar_init(bar(B_QEMPTY), 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(bar(B_KFULL + s), kQuant ? 33 : 1);
+      mbar_init(bar(B_KEMPTY + s), kQuant ? 128 : 1);
+      mbar_init(bar(B_VFULL + s), 1);
+      mbar_init(bar(B_VEMPTY + s), kQuant ? 128 : 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(bar(B_CK + 2 * x), 128);
+      mbar_init(bar(B_CK + 2 * x + 1), 1);
+      mbar_init(bar(B_SREADY + x), 1);
+      mbar_init(bar(B_PREADY + x), 4);
+      mbar_init(bar(B_OREADY + x), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + P::kOffMisc), "r"(P::kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 160) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
+  }
+  if (!kQuant && a.tile_keys < TK) {  // rows that no box reaches: zero V, finite K
+    for (int x = threadIdx.x; x < 2 * NS * P::kStage / 16; x += P::kThreads) reinterpret_cast<uint4*>(smem + P::kOffK)[x] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  block_cut<P::kThreads>(a, cut);  // ends with a barrier
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + P::kOffMisc);
+
+  Walk w;
+  w.init(a, cut);
+  // Keys of tile t (the rest of its rows are masked): whole pages of a sequence, or a part of one page.
+  auto keys_of = [&](int32_t t, int32_t& first_page, int32_t& slot) -> int {
+    int32_t left;
+    if (a.page_tiles) {
+      first_page = t / a.page_tiles;
+      slot = (t - first_page * a.page_tiles) * TK;
+      left = min(w.len - first_page * ps, ps) - slot;
+    } else {
+      first_page = t * n_pages_tile;
+      slot = 0;
+      left = w.len - t * a.tile_keys;
+    }
+    return min(left, a.tile_keys);
+  };
+
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kRegsAux));
+    if (warp == 4 || warp == 6) {
+      // =============================== TMA producers: warp 4 K, masks and scales, warp 6 V ===============================
+      const bool is_k = warp == 4;
+      const CUtensorMap* tm = is_k ? &tmK : &tmV;
+      const int full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY, off = is_k ? P::kOffK : P::kOffV;
+      // page (within a tile) and slot of this lane's two keys
+      int key_page[2], key_slot[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key = lane + 32 * x;
+        key_page[x] = a.page_tiles ? 0 : key / ps;
+        key_slot[x] = key - key_page[x] * (a.page_tiles ? 0 : ps);
+      }
+      const uint32_t tile_bytes = (uint32_t)(a.page_tiles ? TK : ps) * (kQuant ? DP : 128 * P::kChunks) * n_pages_tile;
+      uint32_t jj = 0;
+      bool ok = true;
+      while (ok && w.next(a)) {
+        const int32_t* table = a.c.table + (int64_t)w.b * a.c.table_width;
+        auto pages_at = [&](int32_t i) -> int32_t { return i + lane < a.c.table_width ? __ldg(table + i + lane) : -1; };
+        int32_t base, slot;
+        keys_of(w.t0, base, slot);
+        int32_t cur = pages_at(base), nxt = pages_at(base + 32);
+        for (int32_t t = w.t0; t < w.t0 + w.n; ++t, ++jj) {
+          int32_t first;
+          const int n = keys_of(t, first, slot);
+          if (first >= base + 32) {
+            cur = nxt;
+            base += 32;
+            nxt = pages_at(base + 32);
+          }
+          const int st = jj % NS;
+          ok = __all_sync(kFullMask, mbar_wait(bar(empty + st), ((jj / NS) & 1) ^ 1u, abort_flag, err, is_k ? 111 : 112));
+          if (!ok) break;
+          const int at = first - base;
+          if (is_k) {
+            uint64_t mask = n >= 64 ? ~0ull : (1ull << n) - 1;
+            for (int i = 0; i < n_pages_tile; ++i) {
+              const int32_t page = __shfl_sync(kFullMask, cur, at + i);
+              if (page >= 0 && page < a.c.n_pages) continue;
+              if (a.page_tiles) mask = 0;
+              else mask &= ~(((1ull << ps) - 1) << (i * ps));
+            }
+            if (lane == 0) ring_mask[jj % P::kRing] = mask;
+            if constexpr (kQuant) {
+              float* dst = ring_scale + (jj % P::kRing) * 2 * TK;
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const int key = lane + 32 * x;
+                const int32_t page = __shfl_sync(kFullMask, cur, at + (key_page[x] < n_pages_tile ? key_page[x] : 0));
+                if ((mask >> key) & 1) {
+                  cp_async4(smem_u32(dst + key), a.c.K.scale + a.c.K.scale_at(page, slot + key_slot[x], w.h));
+                  cp_async4(smem_u32(dst + TK + key), a.c.V.scale + a.c.V.scale_at(page, slot + key_slot[x], w.h));
+                } else {
+                  dst[key] = dst[TK + key] = 0.f;
+                }
+              }
+              cp_async_arrive(bar(B_KFULL + st));
+              __syncwarp();
+            }
+          }
+          if (lane == 0) mbar_expect_tx(bar(full + st), tile_bytes);
+          for (int i = 0; i < n_pages_tile; ++i) {
+            int32_t page = __shfl_sync(kFullMask, cur, at + i);
+            if (page < 0 || page >= a.c.n_pages) page = (int32_t)a.c.n_pages;  // behind the last page: zeros
+            if (lane == 0) {
+              if constexpr (kQuant) {
+                tma_load_4d(sbase + off + st * P::kStage + i * ps * DP, tm, 0, slot, w.h, page, bar(full + st));
+              } else {
+#pragma unroll
+                for (int c = 0; c < P::kChunks; ++c)
+                  tma_load_4d(sbase + off + st * P::kStage + c * P::kKVChunk + i * ps * 128, tm, c * 64, slot, w.h, page, bar(full + st));
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      if constexpr (kQuant) asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 5) {
+      // =============================== MMA issuer ===============================
+      const bool el = elect_one();
+      auto wait = [&](int b, uint32_t parity, int code) -> bool { return __all_sync(kFullMask, mbar_wait(bar(b), parity, abort_flag, err, code)); };
+      constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
+      const uint64_t qd = smem_desc(sbase + P::kOffQ, 16, 1024, kLayoutSw128);
+      uint32_t jj = 0, unit = 0;
+      bool ok = true;
+      while (ok && w.next(a)) {
+        const int32_t n = w.n;
+        const bool split = w.tokens * a.group <= P::kRows;
+        ok = wait(B_QFULL, unit & 1, 211);
+        ++unit;
+        if (!ok) break;
+        auto issue_S = [&](int32_t t) -> bool {
+          if (t >= n) return true;
+          const uint32_t j = jj + (uint32_t)t;
+          const int st = kQuant ? 0 : j % NS;
+          if (!wait(kQuant ? B_CK : B_KFULL + st, kQuant ? (j & 1) : ((j / NS) & 1), 212)) return false;
+          tc_fence_after();
+          const uint64_t kd = smem_desc(sbase + (kQuant ? P::kOffCK : P::kOffK + st * P::kStage), 16, 1024, kLayoutSw128);
+          if (el) {
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {  // 16 elements (32 bytes) of the contraction per MMA
+              const int c = kk / 4, in = kk % 4 * 32;
+              mma16_ss(tmem + P::kColS + TK * (j & 1), qd + (uint64_t)((c * P::kQChunk + in) >> 4),
+                       kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS, kk ? 1u : 0u);
+            }
+            tc_commit(bar(B_SREADY + (j & 1)));
+            tc_commit(bar(kQuant ? B_CK + 1 : B_KEMPTY + st));
+            if (t == n - 1) tc_commit(bar(B_QEMPTY));
+          }
+          __syncwarp();
+          return true;
+        };
+        ok = issue_S(0) && issue_S(1);
+        for (int32_t t = 0; t < n && ok; ++t) {
+          const uint32_t j = jj + (uint32_t)t;
+          const int st = kQuant ? 0 : j % NS;
+          ok = wait(B_PREADY + (j & 1), (j >> 1) & 1, 213) && wait(kQuant ? B_CV : B_VFULL + st, kQuant ? (j & 1) : ((j / NS) & 1), 214);
+          if (!ok) break;
+          const uint32_t v_at = sbase + (kQuant ? P::kOffCV : P::kOffV + st * P::kStage);
+          if constexpr (!kQuant) {  // rows behind the sequence's end hold anything, and 0 times anything may be NaN
+            int32_t first, slot;
+            const int keys = keys_of(w.t0 + t, first, slot);
+            if (keys < a.tile_keys) {
+              for (int x = keys * 8 + lane; x < TK * 8; x += 32)
+#pragma unroll
+                for (int c = 0; c < P::kChunks; ++c)
+                  *reinterpret_cast<uint4*>(smem + P::kOffV + st * P::kStage + c * P::kKVChunk + x * 16) = make_uint4(0, 0, 0, 0);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+            }
+          }
+          tc_fence_after();
+          // 16 keys per MMA = two 8-row swizzle groups; 64 columns of d lie kKVChunk apart
+          const uint64_t vd = smem_desc(v_at, P::kKVChunk, 1024, kLayoutSw128);
+          if (el) {
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk)
+              mma16_ts(tmem + P::kColO, tmem + P::kColS + TK * (j & 1) + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO,
+                       kk ? 1u : (t > 0 ? 1u : 0u));
+            if (kMaySplit && split) {
+#pragma unroll
+              for (int kk = 0; kk < TK / 16; ++kk)
+                mma16_ts(tmem + P::kColO, tmem + P::kColS + TK * (j & 1) + TK / 2 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4),
+                         kIdescO, 1u);
+            }
+            tc_commit(bar(B_OREADY + (j & 1)));
+            tc_commit(bar(kQuant ? B_CV + 1 : B_VEMPTY + st));
+          }
+          __syncwarp();
+          ok = issue_S(t + 2);  // its S buffer is free once the product above is queued (the pipe runs them in order)
+        }
+        jj += (uint32_t)n;
+      }
+    } else if (warp >= 8 || !kQuant) {
+      // =============================== Q, and the tiles of an 8-bit cache ===============================
+      constexpr int QT = P::kQThreads;
+      const int tid = threadIdx.x - (kQuant ? 256 : 224);
+      uint32_t jj = 0, unit = 0;
+      bool ok = true;
+      while (ok && w.next(a)) {
+        const int rows = w.rows(a);
+        ok = unit == 0 || mbar_wait(bar(B_QEMPTY), (unit - 1) & 1, abort_flag, err, 411);
+        ok = __all_sync(kFullMask, ok);
+        if (!ok) break;
+        // rows beyond the unit's keep what was there: no row's result depends on another's
+        constexpr int UPR = DP / 8;
+#pragma unroll 4
+        for (int x = tid; x < ((rows * UPR + QT - 1) & ~(QT - 1)); x += QT) {
+          const int r = x / UPR, u = x % UPR;
+          const bool some = r < rows && u * 8 < a.c.d;
+          uint4 q = make_uint4(0, 0, 0, 0);
+          if (some) {
+            const int32_t xr = w.row0 + r, t = xr / a.group;
+            q = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
+                                                ((int64_t)w.h * a.group + (xr - t * a.group)) * a.q_stride[1] + u * 8);
+          }
+          if constexpr (kQuant) {
+            uint32_t v[4] = {q.x, q.y, q.z, q.w};
+            float inv = 1.f;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // times 2^(14 - exponent of the row's largest element)
+              uint32_t top = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) top = max(top, max((v[i] & 0x7fffu) << 16, v[i] & 0x7fff0000u));
+#pragma unroll
+              for (int o = UPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFullMask, top, o));
+              int e = (int)(top >> 23) - 127;
+              e = e > 127 ? 14 : (e < -100 ? -100 : e);  // not finite: as it is
+              const float f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+              inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 y = Half16<__nv_bfloat16>::up(v[i]);
+                v[i] = Half16<__half>::down(y.x * f, y.y * f);
+              }
+            }
+            if constexpr (Widen<TC>::kSwap) {
+#pragma unroll
+              for (int i = 0; i < 4; i += 2) {
+                const uint32_t lo = v[i], hi = v[i + 1];
+                v[i] = (lo & 0xffffu) | (hi << 16);
+                v[i + 1] = (lo >> 16) | (hi & 0xffff0000u);
+              }
+            }
+            q = make_uint4(v[0], v[1], v[2], v[3]);
+            if (u == 0 && r < rows) q_inv[(unit & 1) * P::kRows + r] = inv;
+          }
+          if (r < rows) *reinterpret_cast<uint4*>(smem + P::kOffQ + (u / 8) * P::kQChunk + P::unit(r, u % 8)) = q;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(bar(B_QFULL));
+        ++unit;
+        if constexpr (kQuant) {
+          constexpr int UPT = DP / 16;  // 16-byte units of a row of codes
+          // K one tile ahead of V: S runs ahead of P V
+          auto convert = [&](int32_t t, bool is_v) -> bool {
+            const uint32_t j = jj + (uint32_t)t;
+            const int st = j % NS, full = is_v ? B_VFULL : B_KFULL, done = is_v ? B_CV : B_CK;
+            if (!__all_sync(kFullMask, mbar_wait(bar(full + st), (j / NS) & 1, abort_flag, err, 412) &&
+                                           mbar_wait(bar(done + 1), (j & 1) ^ 1u, abort_flag, err, 413)))
+              return false;
+            int keys = TK;
+            if (is_v) {  // rows behind the sequence's end hold anything
+              int32_t first, slot;
+              keys = keys_of(w.t0 + t, first, slot);
+            }
+            const uint8_t* src = smem + (is_v ? P::kOffV : P::kOffK) + st * P::kStage;
+            uint8_t* dst = smem + (is_v ? P::kOffCV : P::kOffCK);
+#pragma unroll
+            for (int i = 0; i < TK * UPT / QT; ++i) {
+              const int x = i * QT + tid, r = x / UPT, u = x % UPT;
+              uint4 c = *reinterpret_cast<const uint4*>(src + x * 16);
+              if (r >= keys) c = make_uint4(0, 0, 0, 0);
+              uint4 y0, y1;
+              Widen<TC>::four(c.x, y0.x, y0.y);
+              Widen<TC>::four(c.y, y0.z, y0.w);
+              Widen<TC>::four(c.z, y1.x, y1.y);
+              Widen<TC>::four(c.w, y1.z, y1.w);
+              // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
+              const int ch = u / 4, u0 = (u % 4) * 2, s = ch & 1;
+              uint8_t* p = dst + ch * P::kKVChunk;
+              *reinterpret_cast<uint4*>(p + P::unit(r, u0 + s)) = s ? y1 : y0;
+              *reinterpret_cast<uint4*>(p + P::unit(r, u0 + (s ^ 1))) = s ? y0 : y1;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(bar(done));
+            mbar_arrive(bar((is_v ? B_VEMPTY : B_KEMPTY) + st));
+            return true;
+          };
+          ok = convert(0, false);
+          for (int32_t t = 0; t < w.n && ok; ++t) {
+            if (t + 1 < w.n) ok = convert(t + 1, false);
+            ok = ok && convert(t, true);
+          }
+        }
+        jj += (uint32_t)w.n;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kRegsSoftmax));
+    // =============================== softmax: one thread owns one query row ===============================
+    // The reference of a row moves only when its maximum outgrows it by 2^kSlack. float16 probabilities are lifted by 2^kLift (the
+    // largest, times a scale below 2 relative to the scales' reference, is below 2^15): they keep 11 bits down to 2^-24 of the
+    // reference and steps of 2^-34 below, so that a million small ones lose less than 2^-15 of V's magnitude.
+    constexpr bool kHalfP = std::is_same<TP, __half>::value;
+    constexpr float kSlack = kHalfP ? 4.f : 8.f, kLift = kHalfP ? 10.f : 0.f;
+    const uint64_t minus1 = pack2(-1.f, -1.f);
+    constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included
+    const int row = threadIdx.x;
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    const uint32_t tO = tmem + lane_base + P::kColO;
+    uint32_t jj = 0, unit = 0;
+    bool ok = true;
+    while (ok && w.next(a)) {
+      const int rows = w.rows(a);
+      if (warp * 32 >= rows) {  // nothing here: keep step with the barriers
+        for (int32_t t = 0; t < w.n && ok; ++t, ++jj) {
+          ok = __all_sync(kFullMask, mbar_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315));
+          if (ok && lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+        }
+        ++unit;
+        continue;
+      }
+      float m_true = neg_inf(), shift = neg_inf(), sc = a.scale_log2e;
+      uint64_t l2[2] = {0ull, 0ull};
+      const bool split = kMaySplit && w.tokens * a.group <= P::kRows;
+      uint32_t v_exp = 1;  // exponent field of the largest of V's scales so far
+      for (int32_t t = 0; t < w.n; ++t, ++jj) {
+        const uint32_t tS = tmem + lane_base + P::kColS + TK * (jj & 1);
+        ok = __all_sync(kFullMask, mbar_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sr[64];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sr));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
+        const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + jj % P::kRing);
+        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ring_scale + (jj % P::kRing) * 2 * TK);  // K's, then V's
+        float v_move = 1.f;
+        if constexpr (kQuant) {
+          if (t == 0) sc = a.scale_log2e * *reinterpret_cast<volatile float*>(q_inv + (unit & 1) * P::kRows + row);
+          const volatile uint32_t* vs = reinterpret_cast<const volatile uint32_t*>(ks + TK / 4);
+          const uint32_t x = vs[lane] & 0x7fffffffu, y = vs[lane + 32] & 0x7fffffffu;
+          uint32_t top = __reduce_max_sync(kFullMask, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23;
+          if (top > 253) top = 253;
+          if (top > v_exp) {
+            if (t > 0) v_move = exp2f((float)((int)v_exp - (int)top));
+            v_exp = top;
+          }
+        }
+        tc_wait_ld();
+        if constexpr (kQuant) {
+#pragma unroll
+          for (int e = 0; e < 64; e += 4) {
+            const ulonglong2 f = ks[e / 4];
+            float x0, x1, x2, x3;
+            unpack2(fma2(pack2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), f.x, kMinusZero2), x0, x1);
+            unpack2(fma2(pack2(__uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3])), f.y, kMinusZero2), x2, x3);
+            sr[e] = __float_as_uint(x0);
+            sr[e + 1] = __float_as_uint(x1);
+            sr[e + 2] = __float_as_uint(x2);
+            sr[e + 3] = __float_as_uint(x3);
+          }
+        }
+        if (mask != ~0ull) {
+          const uint32_t lo = (uint32_t)mask, hi = (uint32_t)(mask >> 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            sr[e] = ((lo >> e) & 1u) ? sr[e] : 0xff800000u;
+            sr[e + 32] = ((hi >> e) & 1u) ? sr[e + 32] : 0xff800000u;
+          }
+        }
+        float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+        for (int e = 0; e < 64; e += 2)
+          mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], __uint_as_float(sr[e])), __uint_as_float(sr[e + 1]));
+        const float t_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
+        m_true = fmaxf(m_true, t_max);
+        const bool move = t_max > shift + (kSlack + kLift);
+        if (__any_sync(kFullMask, move) || v_move != 1.f) {
+          const float new_shift = move ? t_max - kLift : shift;
+          const float f = move ? ((shift == neg_inf()) ? 0.f : fast_exp2(shift - new_shift)) : 1.0f, fo = f * v_move;
+          const uint64_t f2 = pack2(f, f);
+          l2[0] = fma2(l2[0], f2, 0ull);
+          l2[1] = fma2(l2[1], f2, 0ull);
+          if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
+            ok = __all_sync(kFullMask, mbar_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t ob[8];
+#pragma unroll 1
+            for (int c = 0; c < DP / 8; ++c) {
+              tmem_ld8(tO + c * 8, ob);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * fo);
+              tmem_st8(tO + c * 8, ob);
+            }
+          }
+          shift = new_shift;
+        }
+        const float neg_shift = (shift == neg_inf()) ? 0.f : -shift;
+        const uint64_t ns2 = pack2(neg_shift, neg_shift), sc2 = pack2(sc, sc);
+        const float v_inv = __uint_as_float((254u - v_exp) << 23);
+        const uint64_t vi2 = pack2(v_inv, v_inv);
+        // (first term, and with kLo the second: what the rounding left)
+        auto probabilities = [&](auto lo_tag) {
+          constexpr bool kLo = decltype(lo_tag)::value;
+          uint32_t hi[32], lo[kLo ? 32 : 1];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, ns2), x0, x1);
+            uint64_t p = pack2(fast_exp2(x0), fast_exp2(x1));
+            l2[e & 1] = add2(l2[e & 1], p);
+            if constexpr (kQuant) {
+              const ulonglong2 f = ks[TK / 4 + e / 2];
+              p = fma2(fma2(p, e & 1 ? f.y : f.x, kMinusZero2), vi2, kMinusZero2);
+            }
+            float p0, p1;
+            unpack2(p, p0, p1);
+            hi[e] = Half16<TP>::down(p0, p1);
+            if constexpr (kLo) {
+              const float2 h = Half16<TP>::up(hi[e]);
+              unpack2(fma2(pack2(h.x, h.y), minus1, p), p0, p1);  // exact
+              lo[e] = Half16<TP>::down(p0, p1);
+            }
+          }
+          tmem_st32(tS, hi);
+          if constexpr (kLo) tmem_st32(tS + 32, lo);
+        };
+        if (kMaySplit && split) probabilities(std::integral_constant<bool, kMaySplit>());
+        else probabilities(std::integral_constant<bool, false>());
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+      }
+      ++unit;
+      if (!ok) break;
+      // ---- the piece's rows leave ----
+      ok = __all_sync(kFullMask, mbar_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314));
+      if (!ok) break;
+      tc_fence_after();
+      float la, lb, lc, ld;
+      unpack2(l2[0], la, lb);
+      unpack2(l2[1], lc, ld);
+      const float l_run = (la + lb) + (lc + ld);
+      const bool store = row < rows;
+      const float rel = (m_true == neg_inf()) ? 0.f : fast_exp2(shift - m_true);
+      const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0 + row, blockIdx.x);
+      if (store) {
+        // a NaN score passes the maximum by and shows in the sum
+        const float m = (l_run != l_run && m_true < __int_as_float(0x7f800000)) ? l_run : m_true;
+        a.ml[out] = make_float2(m, l_run * rel);
+      }
+      float* dst = a.O + out * a.d_pad;
+      const float out_f = kQuant ? rel * __uint_as_float(v_exp << 23) : rel;
+      constexpr int kA = Widen<TC>::kSwap ? 2 : 1, kB = 3 - kA;  // the columns of 1 and 2
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t ob[32];
+        tmem_ld32(tO + c * 32, ob);
+        tc_wait_ld();
+        if constexpr (kMaySplit && !kQuant) {
+          uint64_t zero[2] = {0ull, 0ull};  // stay 0 while every value is finite
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            zero[(e >> 1) & 1] = fma2(pack2(__uint_as_float(ob[e]), __uint_as_float(ob[e + 1])), 0ull, zero[(e >> 1) & 1]);
+          if (split && __any_sync(kFullMask, store && ((zero[0] | zero[1]) & 0x7fffffff7fffffffull) != 0ull)) {
+            int32_t first, last, slot, end_slot;
+            keys_of(w.t0, first, slot);
+            const int left = keys_of(w.t0 + w.n - 1, last, end_slot);
+            const int found = infinity_of<T>(a, w.b, w.h, first * ps + slot, last * ps + end_slot + left, c * 32 + lane);
+            for (int e = 0; e < 32; ++e) {
+              const int f = __shfl_sync(kFullMask, found, e);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i == e && f != 0 && l_run == l_run)
+                  ob[i] = f == 2 ? 0x7fc00000u : f > 0 ? 0x7f800000u : 0xff800000u;
+            }
+          }
+        }
+        if (store) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 y = make_float4(__uint_as_float(ob[e]) * out_f, __uint_as_float(ob[e + kA]) * out_f,
+                                         __uint_as_float(ob[e + kB]) * out_f, __uint_as_float(ob[e + 3]) * out_f);
+            if (c * 32 + e < a.d_pad) *reinterpret_cast<float4*>(dst + c * 32 + e) = y;
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+    }
+  }
+
+  // ---- common exit: everyone is done with TMEM before it is released ----
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    if (*abort_flag && lane == 0) {  // copies that may still be in flight land before the CTA's shared memory is reused
+      const uint64_t t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
+      }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::kTmemCols) : "memory");
+  }
+}
+
+}  // namespace tree
+}  // namespace spfa

@@ -365,3 +365,63 @@ def test_refusals(pkg):
     none = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device="cuda")
     fwd(none, *a, torch.zeros(3, dtype=torch.int32, device="cuda"), mk[:0], m[:0], l[:0], none)
     assert pkg.capi.last_device_error() == 0
+
+
+def test_which_kernel_takes_a_call(pkg):
+    """The tensor-core path takes 16-bit calls on rows and pages that the copy engine can address; the others go without."""
+    tiled = pkg.capi.PATH_TILED
+    for dtype, cache, d, page, shift, want in (("bf16", "native", 128, 16, 0, True), ("f16", "native", 40, 8, 0, True),
+                                               ("f16", "int8", 80, 24, 0, True), ("bf16", "e4m3", 64, 100, 0, True),
+                                               ("bf16", "e4m3", 64, 20, 0, False), ("bf16", "e4m3", 40, 16, 0, False),
+                                               ("bf16", "native", 64, 65, 0, True), ("bf16", "native", 136, 16, 0, False),
+                                               ("bf16", "native", 64, 16, 1, False), ("f32", "int8", 64, 16, 0, False)):
+        c, Q, cu, mask = problem(dtype, cache, [70], [2], 2, 1, d, page, shift=shift)
+        run(pkg, c, Q, cu, mask)
+        assert (pkg.capi.last_path() == tiled) == want, (dtype, cache, d, page, shift)
+        pkg.capi.set_path(tiled)
+        try:
+            if want:
+                run(pkg, c, Q, cu, mask)
+            else:
+                with pytest.raises(RuntimeError):
+                    run(pkg, c, Q, cu, mask)
+        finally:
+            pkg.capi.set_path(pkg.capi.PATH_AUTO)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("cache", ["e4m3", "int8"])
+def test_every_code_is_taken_as_its_value(pkg, cache, dtype):
+    """One committed key: O is its V row, whatever the score, and the score is q . k. All 256 codes, on both paths; NaN codes make
+    NaN of their column of O, and as K of the whole row."""
+    codes = torch.arange(256, dtype=torch.uint8).view(4, 64)
+    c, Q, cu, mask = problem(dtype, cache, [1], [1], 4, 4, 64, 16)
+    at = c.place(0, 0)
+    none = torch.zeros(1, 0, dtype=torch.bool)
+    value = torch.from_numpy(np.concatenate([cache_ref.E4M3, [np.nan], -cache_ref.E4M3, [np.nan]])) if cache == "e4m3" else \
+        codes.view(torch.int8).double().flatten()
+    raw = lambda t: t.view(torch.uint8)  # noqa: E731
+    raw(c.V)[at] = codes.cuda()
+    raw(c.K)[at] = 0x18
+    c.V_scale[at], c.K_scale[at] = 2.0 ** -9, 0.25
+    for tag, (m, l, O) in both_paths(pkg, c, Q, cu, none):
+        # the reference of the row is its score rounded to float32, the exponent its unrounded product less that: |x| <= |m log2 e| 2^-24,
+        # and l = 2^x, from an instruction good to 2^-22
+        assert ((l.cpu() - 1).abs() <= m.cpu().abs() * 2.0 ** -24 + 2.0 ** -22).all()
+        assert torch.equal(O.cpu()[0].nan_to_num(7), (value.view(4, 64) * 2.0 ** -9).to(DT[dtype]).nan_to_num(7)), tag
+    raw(c.V)[at] = 1
+    Q = torch.zeros(1, 4, 64, dtype=DT[dtype])
+    for e in range(64):  # m is one code of each head at a time
+        Q.zero_()
+        Q[0, :, e] = 8
+        raw(c.K)[at] = codes.cuda()
+        if cache == "e4m3":
+            raw(c.K)[at][codes.cuda() % 128 == 127] = 0
+        for tag, (m, l, O) in both_paths(pkg, c, Q, cu, none):
+            want = value.view(4, 64)[:, e].nan_to_num(0) * 0.25  # 8 / sqrt(64) = 1
+            assert np.allclose(m.cpu()[0].double(), want, rtol=2.0 ** -22, atol=0), (tag, e)
+    if cache == "e4m3":
+        raw(c.K)[at][2, 5] = 0xff
+        for tag, (m, l, O) in both_paths(pkg, c, Q, cu, none):
+            bad = torch.tensor([[False, False, True, False]])
+            assert torch.equal(torch.isnan(m.cpu()), bad) and torch.equal(torch.isnan(O.cpu()).all(-1), bad), tag
