@@ -15,8 +15,7 @@
 //   warp 7     Q
 //   warps 8-11 (8-bit caches) the conversion of each tile to 16 bits, and Q instead of warp 7
 // An 8-bit tile meets the tensor cores as float16 numbers that equal its codes (11 bits hold e4m3 and int8). The rows' scales stay in
-// fp32: K's multiplies the score, V's the probability before that is rounded, relative to the largest of the scales so far (a power
-// of two that the accumulator gives up when it grows). bfloat16 Q rows become float16 times a power of two: none of their 8 bits is
+// fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the largest of them in. bfloat16 Q rows become float16 times a power of two: none of their 8 bits is
 // lost above 2^-29 of the row's largest element, and below nothing that a float32 sum of the products would show.
 // P is rounded to 16 bits. Where that alone would be as large as the rounding of the result (all but 8-bit caches under bfloat16 Q),
 // units of a single row tile carry a second 16-bit term, the rounding's remainder: they wait for memory, and the second product is
@@ -59,6 +58,37 @@ struct PlanTree {
   static __device__ __forceinline__ uint32_t unit(int row, int u) { return (uint32_t)(row * 128 + ((u ^ (row & 7)) << 4)); }
 };
 
+// mbar_wait of tile_kernels_sm100.cuh with a time hint: a warp of this kernel often waits for several tiles' worth of other roles, and a
+// waiting warp that polls takes issue slots from them.
+__device__ __forceinline__ bool mbar_try_for(uint32_t bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
+// All lanes of a converged warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  bool done = mbar_try_for(bar, parity, 10000u);
+  if (!__all_sync(kFullMask, done)) {
+    const uint64_t t0 = globaltimer();
+    while (!__all_sync(kFullMask, done = done || mbar_try_for(bar, parity, 10000u))) {
+      const bool late = globaltimer() - t0 > kWaitNs;
+      if (__any_sync(kFullMask, *abort_flag || late)) {
+        if (late) {
+          *abort_flag = 1;
+          atomicCAS(err, 0, code);
+        }
+        return false;
+      }
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm, int32_t x, int32_t y, int32_t z, int32_t w, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -80,10 +110,9 @@ template <class TC> struct Widen {  // a cache that holds its values as they are
 template <> struct Widen<e4m3> {
   static constexpr bool kSwap = false;
   static __device__ __forceinline__ void four(uint32_t w, uint32_t& a, uint32_t& b) {
-    const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const __half2_raw y = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    a = (uint32_t)x.x | ((uint32_t)x.y << 16);
-    b = (uint32_t)y.x | ((uint32_t)y.y << 16);
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(w));
   }
 };
 template <> struct Widen<int8_t> {
@@ -203,50 +232,56 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       const bool is_k = warp == 4;
       const CUtensorMap* tm = is_k ? &tmK : &tmV;
       const int full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY, off = is_k ? P::kOffK : P::kOffV;
+      const bool el = elect_one();
       // page (within a tile) and slot of this lane's two keys
       int key_page[2], key_slot[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int key = lane + 32 * x;
-        key_page[x] = a.page_tiles ? 0 : key / ps;
-        key_slot[x] = key - key_page[x] * (a.page_tiles ? 0 : ps);
+        key_page[x] = a.page_tiles ? 0 : min(key / ps, n_pages_tile - 1);
+        key_slot[x] = key - key_page[x] * ps;
       }
       const uint32_t tile_bytes = (uint32_t)(a.page_tiles ? TK : ps) * (kQuant ? DP : 128 * P::kChunks) * n_pages_tile;
+      const uint32_t every = 0xffffffffu >> (32 - n_pages_tile);
       uint32_t jj = 0;
       bool ok = true;
       while (ok && w.next(a)) {
         const int32_t* table = a.c.table + (int64_t)w.b * a.c.table_width;
         auto pages_at = [&](int32_t i) -> int32_t { return i + lane < a.c.table_width ? __ldg(table + i + lane) : -1; };
-        int32_t base, slot;
-        keys_of(w.t0, base, slot);
-        int32_t cur = pages_at(base), nxt = pages_at(base + 32);
-        for (int32_t t = w.t0; t < w.t0 + w.n; ++t, ++jj) {
-          int32_t first;
-          const int n = keys_of(t, first, slot);
+        int32_t first, slot;  // of the tile
+        keys_of(w.t0, first, slot);
+        int32_t base = first, nxt = pages_at(base), cur = 0;
+        uint32_t valid = 0;
+        auto turn = [&](int32_t more) {  // the next 32 pages; pages that do not exist become the one behind the last: zeros
+          const bool in = nxt >= 0 && nxt < a.c.n_pages;
+          valid = __ballot_sync(kFullMask, in);
+          cur = in ? nxt : (int32_t)a.c.n_pages;
+          nxt = pages_at(more);
+        };
+        turn(base + 32);
+        for (int32_t t = 0; t < w.n; ++t, ++jj) {
           if (first >= base + 32) {
-            cur = nxt;
             base += 32;
-            nxt = pages_at(base + 32);
+            turn(base + 32);
           }
           const int st = jj % NS;
-          ok = __all_sync(kFullMask, mbar_wait(bar(empty + st), ((jj / NS) & 1) ^ 1u, abort_flag, err, is_k ? 111 : 112));
+          ok = warp_wait(bar(empty + st), ((jj / NS) & 1) ^ 1u, abort_flag, err, is_k ? 111 : 112);
           if (!ok) break;
           const int at = first - base;
           if (is_k) {
+            const int n = min(a.page_tiles ? min(w.len - first * ps, ps) - slot : w.len - (w.t0 + t) * a.tile_keys, a.tile_keys);
             uint64_t mask = n >= 64 ? ~0ull : (1ull << n) - 1;
-            for (int i = 0; i < n_pages_tile; ++i) {
-              const int32_t page = __shfl_sync(kFullMask, cur, at + i);
-              if (page >= 0 && page < a.c.n_pages) continue;
-              if (a.page_tiles) mask = 0;
-              else mask &= ~(((1ull << ps) - 1) << (i * ps));
+            if (((valid >> at) & every) != every) {
+              for (int i = 0; i < n_pages_tile; ++i)
+                if (!((valid >> (at + i)) & 1u)) mask &= a.page_tiles ? 0ull : ~(((1ull << ps) - 1) << (i * ps));
             }
-            if (lane == 0) ring_mask[jj % P::kRing] = mask;
+            if (el) ring_mask[jj % P::kRing] = mask;
             if constexpr (kQuant) {
               float* dst = ring_scale + (jj % P::kRing) * 2 * TK;
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 const int key = lane + 32 * x;
-                const int32_t page = __shfl_sync(kFullMask, cur, at + (key_page[x] < n_pages_tile ? key_page[x] : 0));
+                const int64_t page = __shfl_sync(kFullMask, cur, at + key_page[x]);
                 if ((mask >> key) & 1) {
                   cp_async4(smem_u32(dst + key), a.c.K.scale + a.c.K.scale_at(page, slot + key_slot[x], w.h));
                   cp_async4(smem_u32(dst + TK + key), a.c.V.scale + a.c.V.scale_at(page, slot + key_slot[x], w.h));
@@ -258,28 +293,37 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               __syncwarp();
             }
           }
-          if (lane == 0) mbar_expect_tx(bar(full + st), tile_bytes);
+          if (el) mbar_expect_tx(bar(full + st), tile_bytes);
+          uint32_t to = sbase + off + st * P::kStage;
           for (int i = 0; i < n_pages_tile; ++i) {
-            int32_t page = __shfl_sync(kFullMask, cur, at + i);
-            if (page < 0 || page >= a.c.n_pages) page = (int32_t)a.c.n_pages;  // behind the last page: zeros
-            if (lane == 0) {
+            const int32_t page = __shfl_sync(kFullMask, cur, at + i);
+            if (el) {
               if constexpr (kQuant) {
-                tma_load_4d(sbase + off + st * P::kStage + i * ps * DP, tm, 0, slot, w.h, page, bar(full + st));
+                tma_load_4d(to, tm, 0, slot, w.h, page, bar(full + st));
               } else {
 #pragma unroll
-                for (int c = 0; c < P::kChunks; ++c)
-                  tma_load_4d(sbase + off + st * P::kStage + c * P::kKVChunk + i * ps * 128, tm, c * 64, slot, w.h, page, bar(full + st));
+                for (int c = 0; c < P::kChunks; ++c) tma_load_4d(to + c * P::kKVChunk, tm, c * 64, slot, w.h, page, bar(full + st));
               }
             }
+            to += ps * (kQuant ? DP : 128);
           }
           __syncwarp();
+          if (a.page_tiles) {
+            slot += TK;
+            if (slot >= ps) {
+              slot = 0;
+              ++first;
+            }
+          } else {
+            first += n_pages_tile;
+          }
         }
       }
       if constexpr (kQuant) asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 5) {
       // =============================== MMA issuer ===============================
       const bool el = elect_one();
-      auto wait = [&](int b, uint32_t parity, int code) -> bool { return __all_sync(kFullMask, mbar_wait(bar(b), parity, abort_flag, err, code)); };
+      auto wait = [&](int b, uint32_t parity, int code) -> bool { return warp_wait(bar(b), parity, abort_flag, err, code); };
       constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
       const uint64_t qd = smem_desc(sbase + P::kOffQ, 16, 1024, kLayoutSw128);
       uint32_t jj = 0, unit = 0;
@@ -360,8 +404,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       bool ok = true;
       while (ok && w.next(a)) {
         const int rows = w.rows(a);
-        ok = unit == 0 || mbar_wait(bar(B_QEMPTY), (unit - 1) & 1, abort_flag, err, 411);
-        ok = __all_sync(kFullMask, ok);
+        ok = unit == 0 || warp_wait(bar(B_QEMPTY), (unit - 1) & 1, abort_flag, err, 411);
         if (!ok) break;
         // rows beyond the unit's keep what was there: no row's result depends on another's
         constexpr int UPR = DP / 8;
@@ -411,46 +454,41 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         mbar_arrive(bar(B_QFULL));
         ++unit;
         if constexpr (kQuant) {
-          constexpr int UPT = DP / 16;  // 16-byte units of a row of codes
-          // K one tile ahead of V: S runs ahead of P V
-          auto convert = [&](int32_t t, bool is_v) -> bool {
+          // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1)
+          constexpr int UPT = DP / 16, R = QT / UPT;  // 16-byte units of a row of codes, rows of one step
+          const int r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
+          // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
+          const uint32_t to0 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + s), to1 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + (s ^ 1));
+          for (int32_t step = 0; step < 2 * w.n && ok; ++step) {
+            const bool is_v = step > 0 && ((step & 1) == 0 || step == 2 * w.n - 1);
+            const int32_t t = step == 2 * w.n - 1 ? w.n - 1 : (step + 1) / 2 - (is_v ? 1 : 0);
             const uint32_t j = jj + (uint32_t)t;
-            const int st = j % NS, full = is_v ? B_VFULL : B_KFULL, done = is_v ? B_CV : B_CK;
-            if (!__all_sync(kFullMask, mbar_wait(bar(full + st), (j / NS) & 1, abort_flag, err, 412) &&
-                                           mbar_wait(bar(done + 1), (j & 1) ^ 1u, abort_flag, err, 413)))
-              return false;
-            int keys = TK;
-            if (is_v) {  // rows behind the sequence's end hold anything
+            const int st = j % NS, done = is_v ? B_CV : B_CK;
+            ok = warp_wait(bar((is_v ? B_VFULL : B_KFULL) + st), (j / NS) & 1, abort_flag, err, 412) &&
+                 warp_wait(bar(done + 1), (j & 1) ^ 1u, abort_flag, err, 413);
+            if (!ok) break;
+            int keys = is_v ? a.tile_keys : TK;  // behind them lies what no box reaches
+            if (is_v && w.t0 + t == w.tiles - 1) {  // rows behind the sequence's end hold anything
               int32_t first, slot;
               keys = keys_of(w.t0 + t, first, slot);
             }
-            const uint8_t* src = smem + (is_v ? P::kOffV : P::kOffK) + st * P::kStage;
+            const uint8_t* src = smem + (is_v ? P::kOffV : P::kOffK) + st * P::kStage + tid * 16;
             uint8_t* dst = smem + (is_v ? P::kOffCV : P::kOffCK);
 #pragma unroll
-            for (int i = 0; i < TK * UPT / QT; ++i) {
-              const int x = i * QT + tid, r = x / UPT, u = x % UPT;
-              uint4 c = *reinterpret_cast<const uint4*>(src + x * 16);
-              if (r >= keys) c = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < TK / R; ++i) {
+              uint4 c = *reinterpret_cast<const uint4*>(src + i * R * DP);
+              if (keys < TK && r0 + i * R >= keys) c = make_uint4(0, 0, 0, 0);
               uint4 y0, y1;
               Widen<TC>::four(c.x, y0.x, y0.y);
               Widen<TC>::four(c.y, y0.z, y0.w);
               Widen<TC>::four(c.z, y1.x, y1.y);
               Widen<TC>::four(c.w, y1.z, y1.w);
-              // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
-              const int ch = u / 4, u0 = (u % 4) * 2, s = ch & 1;
-              uint8_t* p = dst + ch * P::kKVChunk;
-              *reinterpret_cast<uint4*>(p + P::unit(r, u0 + s)) = s ? y1 : y0;
-              *reinterpret_cast<uint4*>(p + P::unit(r, u0 + (s ^ 1))) = s ? y0 : y1;
+              *reinterpret_cast<uint4*>(dst + to0 + i * R * 128) = s ? y1 : y0;
+              *reinterpret_cast<uint4*>(dst + to1 + i * R * 128) = s ? y0 : y1;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             mbar_arrive(bar(done));
             mbar_arrive(bar((is_v ? B_VEMPTY : B_KEMPTY) + st));
-            return true;
-          };
-          ok = convert(0, false);
-          for (int32_t t = 0; t < w.n && ok; ++t) {
-            if (t + 1 < w.n) ok = convert(t + 1, false);
-            ok = ok && convert(t, true);
           }
         }
         jj += (uint32_t)w.n;
@@ -459,9 +497,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kRegsSoftmax));
     // =============================== softmax: one thread owns one query row ===============================
-    // The reference of a row moves only when its maximum outgrows it by 2^kSlack. float16 probabilities are lifted by 2^kLift (the
-    // largest, times a scale below 2 relative to the scales' reference, is below 2^15): they keep 11 bits down to 2^-24 of the
-    // reference and steps of 2^-34 below, so that a million small ones lose less than 2^-15 of V's magnitude.
+    // P = 2^(s - shift). A row's shift is the maximum it was last set at, less kLift, plus the exponent of the largest of V's scales
+    // (8-bit caches, from 2^-80 on): it is set anew only when that outgrows it by kSlack. A float16 probability times its scale is
+    // below 2^(kLift + kSlack + 1) = 2^15 then, keeps 11 bits down to 2^-24 of its reference and steps of 2^-34 below, so that a
+    // million small ones lose less than 2^-15 of V's magnitude.
     constexpr bool kHalfP = std::is_same<TP, __half>::value;
     constexpr float kSlack = kHalfP ? 4.f : 8.f, kLift = kHalfP ? 10.f : 0.f;
     const uint64_t minus1 = pack2(-1.f, -1.f);
@@ -475,7 +514,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       const int rows = w.rows(a);
       if (warp * 32 >= rows) {  // nothing here: keep step with the barriers
         for (int32_t t = 0; t < w.n && ok; ++t, ++jj) {
-          ok = __all_sync(kFullMask, mbar_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315));
+          ok = warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315);
           if (ok && lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
         }
         ++unit;
@@ -484,10 +523,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       float m_true = neg_inf(), shift = neg_inf(), sc = a.scale_log2e;
       uint64_t l2[2] = {0ull, 0ull};
       const bool split = kMaySplit && w.tokens * a.group <= P::kRows;
-      uint32_t v_exp = 1;  // exponent field of the largest of V's scales so far
+      float v_ref = -80.f;  // exponent of the largest of V's scales so far
       for (int32_t t = 0; t < w.n; ++t, ++jj) {
         const uint32_t tS = tmem + lane_base + P::kColS + TK * (jj & 1);
-        ok = __all_sync(kFullMask, mbar_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311));
+        ok = warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311);
         if (!ok) break;
         tc_fence_after();
         uint32_t sr[64];
@@ -495,17 +534,12 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
         const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + jj % P::kRing);
         const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ring_scale + (jj % P::kRing) * 2 * TK);  // K's, then V's
-        float v_move = 1.f;
         if constexpr (kQuant) {
           if (t == 0) sc = a.scale_log2e * *reinterpret_cast<volatile float*>(q_inv + (unit & 1) * P::kRows + row);
           const volatile uint32_t* vs = reinterpret_cast<const volatile uint32_t*>(ks + TK / 4);
           const uint32_t x = vs[lane] & 0x7fffffffu, y = vs[lane + 32] & 0x7fffffffu;
-          uint32_t top = __reduce_max_sync(kFullMask, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23;
-          if (top > 253) top = 253;
-          if (top > v_exp) {
-            if (t > 0) v_move = exp2f((float)((int)v_exp - (int)top));
-            v_exp = top;
-          }
+          const int top = (int)(__reduce_max_sync(kFullMask, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23) - 127;
+          v_ref = fmaxf(v_ref, (float)min(100, top));
         }
         tc_wait_ld();
         if constexpr (kQuant) {
@@ -535,15 +569,16 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], __uint_as_float(sr[e])), __uint_as_float(sr[e + 1]));
         const float t_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
         m_true = fmaxf(m_true, t_max);
-        const bool move = t_max > shift + (kSlack + kLift);
-        if (__any_sync(kFullMask, move) || v_move != 1.f) {
-          const float new_shift = move ? t_max - kLift : shift;
-          const float f = move ? ((shift == neg_inf()) ? 0.f : fast_exp2(shift - new_shift)) : 1.0f, fo = f * v_move;
+        const float want = kQuant ? t_max + (v_ref - kLift) : t_max - kLift;
+        const bool move = want > shift + kSlack;
+        if (__any_sync(kFullMask, move)) {
+          const float new_shift = move ? want : shift;
+          const float f = move ? ((shift == neg_inf()) ? 0.f : fast_exp2(shift - new_shift)) : 1.0f;
           const uint64_t f2 = pack2(f, f);
           l2[0] = fma2(l2[0], f2, 0ull);
           l2[1] = fma2(l2[1], f2, 0ull);
           if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
-            ok = __all_sync(kFullMask, mbar_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312));
+            ok = warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312);
             if (!ok) break;
             tc_fence_after();
             uint32_t ob[8];
@@ -552,7 +587,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               tmem_ld8(tO + c * 8, ob);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * fo);
+              for (int e = 0; e < 8; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * f);
               tmem_st8(tO + c * 8, ob);
             }
           }
@@ -560,8 +595,6 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
         const float neg_shift = (shift == neg_inf()) ? 0.f : -shift;
         const uint64_t ns2 = pack2(neg_shift, neg_shift), sc2 = pack2(sc, sc);
-        const float v_inv = __uint_as_float((254u - v_exp) << 23);
-        const uint64_t vi2 = pack2(v_inv, v_inv);
         // (first term, and with kLo the second: what the rounding left)
         auto probabilities = [&](auto lo_tag) {
           constexpr bool kLo = decltype(lo_tag)::value;
@@ -574,7 +607,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             l2[e & 1] = add2(l2[e & 1], p);
             if constexpr (kQuant) {
               const ulonglong2 f = ks[TK / 4 + e / 2];
-              p = fma2(fma2(p, e & 1 ? f.y : f.x, kMinusZero2), vi2, kMinusZero2);
+              p = fma2(p, e & 1 ? f.y : f.x, kMinusZero2);
             }
             float p0, p1;
             unpack2(p, p0, p1);
@@ -598,7 +631,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       ++unit;
       if (!ok) break;
       // ---- the piece's rows leave ----
-      ok = __all_sync(kFullMask, mbar_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314));
+      ok = warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314);
       if (!ok) break;
       tc_fence_after();
       float la, lb, lc, ld;
@@ -614,7 +647,6 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         a.ml[out] = make_float2(m, l_run * rel);
       }
       float* dst = a.O + out * a.d_pad;
-      const float out_f = kQuant ? rel * __uint_as_float(v_exp << 23) : rel;
       constexpr int kA = Widen<TC>::kSwap ? 2 : 1, kB = 3 - kA;  // the columns of 1 and 2
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
@@ -643,8 +675,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         if (store) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
-            const float4 y = make_float4(__uint_as_float(ob[e]) * out_f, __uint_as_float(ob[e + kA]) * out_f,
-                                         __uint_as_float(ob[e + kB]) * out_f, __uint_as_float(ob[e + 3]) * out_f);
+            const float4 y = make_float4(__uint_as_float(ob[e]) * rel, __uint_as_float(ob[e + kA]) * rel,
+                                         __uint_as_float(ob[e + kB]) * rel, __uint_as_float(ob[e + 3]) * rel);
             if (c * 32 + e < a.d_pad) *reinterpret_cast<float4*>(dst + c * 32 + e) = y;
           }
         }
