@@ -7,13 +7,14 @@
 //   P  = exp2(S c - shift) in registers, one thread a row, rounded to 16 bits and written over S
 //   O += P V_j             128 x DP fp32 in TMEM
 // Rows beyond a unit's are not computed: their warps only keep step. Roles (256 threads):
-//   warps 0-3  softmax and the pieces' epilogue: thread t <-> row t <-> TMEM lane t
+//   warps 0-3  Q, softmax and the pieces' epilogue: thread t <-> row t <-> TMEM lane t
 //   warp 4     TMA producer of K, masks and scales: page numbers 32 at a time in the lanes, one box for each page of a tile and 128
 //              bytes of d. Pages that do not exist are fetched from behind the last one, where the copy engine fills with zeros.
 //   warp 5     MMA issuer
 //   warp 6     TMA producer of V
-//   warp 7     Q
-//   warps 8-11 (8-bit caches) the conversion of each tile to 16 bits, and Q instead of warp 7
+//   warps 8-11 (8-bit caches) the conversion of each tile to 16 bits
+// A unit of at most 64 (32) rows has them two (four) times in Q: each copy takes half (a quarter) of every tile's columns, so that all
+// four softmax warps work, and the copies are added up at the end of the piece.
 // An 8-bit tile meets the tensor cores as float16 numbers that equal its codes (11 bits hold e4m3 and int8). The rows' scales stay in
 // fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the largest of them in. bfloat16 Q rows become float16 times a power of two: none of their 8 bits is
 // lost above 2^-29 of the row's largest element, and below nothing that a float32 sum of the products would show.
@@ -34,7 +35,7 @@ template <int DP, class TC>
 struct PlanTree {
   static constexpr bool kQuant = sizeof(TC) == 1;
   static constexpr int kThreads = kQuant ? 384 : 256, kRegsLaunch = kQuant ? 80 : 128;
-  static constexpr int kRegsSoftmax = kQuant ? 128 : 168, kRegsAux = kQuant ? 56 : 88, kQThreads = kQuant ? 128 : 32;
+  static constexpr int kRegsSoftmax = kQuant ? 128 : 168, kRegsAux = kQuant ? 56 : 88, kConvert = 128;
   static constexpr int kRegsNeeded = kRegsSoftmax * 128 + kRegsAux * (kThreads - 128);
   static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
   static constexpr int TK = 64, kRows = 128, kChunks = DP / 64;
@@ -45,8 +46,8 @@ struct PlanTree {
   static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
   static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStage, kOffCK = kOffV + NS * kStage;
   static constexpr int kOffCV = kOffCK + (kQuant ? kTile : 0), kOffScale = kOffCV + (kQuant ? kTile : 0);
-  static constexpr int kOffQInv = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffQInv + (kQuant ? 2 * kRows * 4 : 0);
-  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 2 + 4 * NS + 4 + 6;
+  static constexpr int kOffRow = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffRow + kRows * 8;
+  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 1 + 4 * NS + 4 + 6;
   static constexpr int kOffCut = kOffBar + kNumBars * 8, kOffMisc = kOffCut + (int)sizeof(Cut);
   static constexpr int kDynSmem = kOffMisc + 16 + 1024;
   static_assert(2 * (kDynSmem + 1024) <= 228 * 1024, "two CTAs share an SM");
@@ -93,6 +94,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
@@ -159,20 +168,19 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + P::kOffBar + 8u * i; };
-  constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = 2 + NS, B_VFULL = 2 + 2 * NS, B_VEMPTY = 2 + 3 * NS,
-                B_CK = 2 + 4 * NS /* full, empty */, B_CV = B_CK + 2, B_SREADY = B_CK + 4, B_PREADY = B_SREADY + 2, B_OREADY = B_SREADY + 4;
+  constexpr int B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 1 + NS, B_VFULL = 1 + 2 * NS, B_VEMPTY = 1 + 3 * NS,
+                B_CK = 1 + 4 * NS /* full, empty */, B_CV = B_CK + 2, B_SREADY = B_CK + 4, B_PREADY = B_SREADY + 2, B_OREADY = B_SREADY + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::kOffMisc + 4);
   Cut* cut = reinterpret_cast<Cut*>(smem + P::kOffCut);
   uint64_t* ring_mask = reinterpret_cast<uint64_t*>(smem + P::kOffMask);
   float* ring_scale = reinterpret_cast<float*>(smem + P::kOffScale);  // [ring][K, V][TK]
-  float* q_inv = reinterpret_cast<float*>(smem + P::kOffQInv);        // [unit parity][row]
+  float2* row_ml = reinterpret_cast<float2*>(smem + P::kOffRow);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int32_t ps = a.c.page_size;
   const int n_pages_tile = a.page_tiles ? 1 : a.tile_keys / ps;  // pages of a tile
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(B_QFULL), P::kQThreads);
-    mbar_init(bar(B_QEMPTY), 1);
+    mbar_init(bar(B_QFULL), 128);
     for (int s = 0; s < NS; ++s) {
       mbar_init(bar(B_KFULL + s), kQuant ? 33 : 1);
       mbar_init(bar(B_KEMPTY + s), kQuant ? 128 : 1);
@@ -350,7 +358,6 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             }
             tc_commit(bar(B_SREADY + (j & 1)));
             tc_commit(bar(kQuant ? B_CK + 1 : B_KEMPTY + st));
-            if (t == n - 1) tc_commit(bar(B_QEMPTY));
           }
           __syncwarp();
           return true;
@@ -396,69 +403,17 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
         jj += (uint32_t)n;
       }
-    } else if (warp >= 8 || !kQuant) {
-      // =============================== Q, and the tiles of an 8-bit cache ===============================
-      constexpr int QT = P::kQThreads;
-      const int tid = threadIdx.x - (kQuant ? 256 : 224);
-      uint32_t jj = 0, unit = 0;
-      bool ok = true;
-      while (ok && w.next(a)) {
-        const int rows = w.rows(a);
-        ok = unit == 0 || warp_wait(bar(B_QEMPTY), (unit - 1) & 1, abort_flag, err, 411);
-        if (!ok) break;
-        // rows beyond the unit's keep what was there: no row's result depends on another's
-        constexpr int UPR = DP / 8;
-#pragma unroll 4
-        for (int x = tid; x < ((rows * UPR + QT - 1) & ~(QT - 1)); x += QT) {
-          const int r = x / UPR, u = x % UPR;
-          const bool some = r < rows && u * 8 < a.c.d;
-          uint4 q = make_uint4(0, 0, 0, 0);
-          if (some) {
-            const int32_t xr = w.row0 + r, t = xr / a.group;
-            q = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
-                                                ((int64_t)w.h * a.group + (xr - t * a.group)) * a.q_stride[1] + u * 8);
-          }
-          if constexpr (kQuant) {
-            uint32_t v[4] = {q.x, q.y, q.z, q.w};
-            float inv = 1.f;
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // times 2^(14 - exponent of the row's largest element)
-              uint32_t top = 0;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) top = max(top, max((v[i] & 0x7fffu) << 16, v[i] & 0x7fff0000u));
-#pragma unroll
-              for (int o = UPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(kFullMask, top, o));
-              int e = (int)(top >> 23) - 127;
-              e = e > 127 ? 14 : (e < -100 ? -100 : e);  // not finite: as it is
-              const float f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-              inv = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 y = Half16<__nv_bfloat16>::up(v[i]);
-                v[i] = Half16<__half>::down(y.x * f, y.y * f);
-              }
-            }
-            if constexpr (Widen<TC>::kSwap) {
-#pragma unroll
-              for (int i = 0; i < 4; i += 2) {
-                const uint32_t lo = v[i], hi = v[i + 1];
-                v[i] = (lo & 0xffffu) | (hi << 16);
-                v[i + 1] = (lo >> 16) | (hi & 0xffff0000u);
-              }
-            }
-            q = make_uint4(v[0], v[1], v[2], v[3]);
-            if (u == 0 && r < rows) q_inv[(unit & 1) * P::kRows + r] = inv;
-          }
-          if (r < rows) *reinterpret_cast<uint4*>(smem + P::kOffQ + (u / 8) * P::kQChunk + P::unit(r, u % 8)) = q;
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bar(B_QFULL));
-        ++unit;
-        if constexpr (kQuant) {
-          // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1)
-          constexpr int UPT = DP / 16, R = QT / UPT;  // 16-byte units of a row of codes, rows of one step
-          const int r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
-          // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
-          const uint32_t to0 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + s), to1 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + (s ^ 1));
+    } else if (kQuant && warp >= 8) {
+      // =============================== the tiles of an 8-bit cache ===============================
+      if constexpr (kQuant) {
+        // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1)
+        constexpr int UPT = DP / 16, R = P::kConvert / UPT;  // 16-byte units of a row of codes, rows of one step
+        const int tid = threadIdx.x - 256, r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
+        // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
+        const uint32_t to0 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + s), to1 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + (s ^ 1));
+        uint32_t jj = 0;
+        bool ok = true;
+        while (ok && w.next(a)) {
           for (int32_t step = 0; step < 2 * w.n && ok; ++step) {
             const bool is_v = step > 0 && ((step & 1) == 0 || step == 2 * w.n - 1);
             const int32_t t = step == 2 * w.n - 1 ? w.n - 1 : (step + 1) / 2 - (is_v ? 1 : 0);
@@ -490,8 +445,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             mbar_arrive(bar(done));
             mbar_arrive(bar((is_v ? B_VEMPTY : B_KEMPTY) + st));
           }
+          jj += (uint32_t)w.n;
         }
-        jj += (uint32_t)w.n;
       }
     }
   } else {
@@ -505,46 +460,113 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     constexpr float kSlack = kHalfP ? 4.f : 8.f, kLift = kHalfP ? 10.f : 0.f;
     const uint64_t minus1 = pack2(-1.f, -1.f);
     constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included
-    const int row = threadIdx.x;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     const uint32_t tO = tmem + lane_base + P::kColO;
-    uint32_t jj = 0, unit = 0;
+    auto group_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    uint32_t jj = 0;
     bool ok = true;
-    while (ok && w.next(a)) {
+
+    // One piece. kCols: the columns of a tile that a thread works on, 64 over the number of copies of the unit's rows.
+    auto piece = [&](auto cols_tag) -> bool {
+      constexpr int kCols = decltype(cols_tag)::value, kCopies = 64 / kCols, kBlock = 128 / kCopies;
       const int rows = w.rows(a);
-      if (warp * 32 >= rows) {  // nothing here: keep step with the barriers
-        for (int32_t t = 0; t < w.n && ok; ++t, ++jj) {
-          ok = warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315);
-          if (ok && lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+      const int row = threadIdx.x % kBlock, copy = threadIdx.x / kBlock, col0 = copy * kCols;  // the copy is the warp's
+      const bool mine = row < rows;
+      // ---- Q: every product with the last unit's has completed ----
+      float sc = a.scale_log2e;
+      if (mine) {
+        const int32_t xr = w.row0 + row, t = xr / a.group;
+        const T* src = reinterpret_cast<const T*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
+                       ((int64_t)w.h * a.group + (xr - t * a.group)) * a.q_stride[1];
+        auto eight = [&](int u0, uint4 (&q)[8]) {  // eight 16-byte units, all in flight together
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            q[i] = make_uint4(0, 0, 0, 0);
+            if ((u0 + i) * 8 < a.c.d) q[i] = __ldg(reinterpret_cast<const uint4*>(src) + u0 + i);
+          }
+        };
+        float f = 1.f;
+        if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {  // times 2^(14 - exponent of the row's largest element)
+          uint32_t top = 0;
+#pragma unroll 1
+          for (int u = 0; u < DP / 8; u += 8) {
+            uint4 q[8];
+            eight(u, q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t x = __vmaxu2(__vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu),
+                                          __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
+              top = max(top, max(x << 16, x & 0xffff0000u));
+            }
+          }
+          int e = (int)(top >> 23) - 127;
+          e = e > 127 ? 14 : (e < -100 ? -100 : e);  // not finite: as it is
+          f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+          sc *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
         }
-        ++unit;
-        continue;
+#pragma unroll 1
+        for (int u = 0; u < DP / 8; u += 8) {
+          uint4 q[8];
+          eight(u, q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+            if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 y = Half16<__nv_bfloat16>::up(v[k]);
+                v[k] = Half16<__half>::down(y.x * f, y.y * f);
+              }
+            }
+            if constexpr (Widen<TC>::kSwap) {
+#pragma unroll
+              for (int k = 0; k < 4; k += 2) {
+                const uint32_t x = v[k], y = v[k + 1];
+                v[k] = (x & 0xffffu) | (y << 16);
+                v[k + 1] = (x >> 16) | (y & 0xffff0000u);
+              }
+            }
+            *reinterpret_cast<uint4*>(smem + P::kOffQ + (u / 8) * P::kQChunk + P::unit(threadIdx.x, i)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }  // rows beyond the unit's keep what was there: no row's result depends on another's
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(bar(B_QFULL));
+      if (kCopies == 1 && warp * 32 >= rows) {  // nothing here: keep step with the barriers
+        for (int32_t t = 0; t < w.n; ++t, ++jj) {
+          if (!warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315)) return false;
+          if (lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+        }
+        return true;
       }
-      float m_true = neg_inf(), shift = neg_inf(), sc = a.scale_log2e;
-      uint64_t l2[2] = {0ull, 0ull};
       const bool split = kMaySplit && w.tokens * a.group <= P::kRows;
+      float m_true = neg_inf(), shift = neg_inf();
       float v_ref = -80.f;  // exponent of the largest of V's scales so far
+      uint64_t l2[2] = {0ull, 0ull};
       for (int32_t t = 0; t < w.n; ++t, ++jj) {
         const uint32_t tS = tmem + lane_base + P::kColS + TK * (jj & 1);
-        ok = warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311);
-        if (!ok) break;
+        if (!warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311)) return false;
         tc_fence_after();
-        uint32_t sr[64];
-        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sr));
-        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
+        uint32_t sr[kCols];
+        if constexpr (kCols == 16) tmem_ld16(tS + col0, sr);
+        if constexpr (kCols == 32) tmem_ld32(tS + col0, sr);
+        if constexpr (kCols == 64) {
+          tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sr));
+          tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
+        }
         const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + jj % P::kRing);
-        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(ring_scale + (jj % P::kRing) * 2 * TK);  // K's, then V's
+        [[maybe_unused]] const float* scales = ring_scale + (jj % P::kRing) * 2 * TK + col0;
+        [[maybe_unused]] const ulonglong2 *ks = reinterpret_cast<const ulonglong2*>(scales), *vs = reinterpret_cast<const ulonglong2*>(scales + TK);
         if constexpr (kQuant) {
-          if (t == 0) sc = a.scale_log2e * *reinterpret_cast<volatile float*>(q_inv + (unit & 1) * P::kRows + row);
-          const volatile uint32_t* vs = reinterpret_cast<const volatile uint32_t*>(ks + TK / 4);
-          const uint32_t x = vs[lane] & 0x7fffffffu, y = vs[lane + 32] & 0x7fffffffu;
+          const volatile uint32_t* all = reinterpret_cast<const volatile uint32_t*>(scales + TK - col0);
+          const uint32_t x = all[lane] & 0x7fffffffu, y = all[lane + 32] & 0x7fffffffu;
           const int top = (int)(__reduce_max_sync(kFullMask, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23) - 127;
           v_ref = fmaxf(v_ref, (float)min(100, top));
         }
         tc_wait_ld();
         if constexpr (kQuant) {
 #pragma unroll
-          for (int e = 0; e < 64; e += 4) {
+          for (int e = 0; e < kCols; e += 4) {
             const ulonglong2 f = ks[e / 4];
             float x0, x1, x2, x3;
             unpack2(fma2(pack2(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), f.x, kMinusZero2), x0, x1);
@@ -556,16 +578,14 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           }
         }
         if (mask != ~0ull) {
-          const uint32_t lo = (uint32_t)mask, hi = (uint32_t)(mask >> 32);
+          const uint64_t here = mask >> col0;
+          const uint32_t lo = (uint32_t)here, hi = (uint32_t)(here >> 32);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            sr[e] = ((lo >> e) & 1u) ? sr[e] : 0xff800000u;
-            sr[e + 32] = ((hi >> e) & 1u) ? sr[e + 32] : 0xff800000u;
-          }
+          for (int e = 0; e < kCols; ++e) sr[e] = (((e < 32 ? lo : hi) >> (e & 31)) & 1u) ? sr[e] : 0xff800000u;
         }
         float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
-        for (int e = 0; e < 64; e += 2)
+        for (int e = 0; e < kCols; e += 2)
           mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], __uint_as_float(sr[e])), __uint_as_float(sr[e + 1]));
         const float t_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
         m_true = fmaxf(m_true, t_max);
@@ -578,8 +598,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           l2[0] = fma2(l2[0], f2, 0ull);
           l2[1] = fma2(l2[1], f2, 0ull);
           if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
-            ok = warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312);
-            if (!ok) break;
+            if (!warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312)) return false;
             tc_fence_after();
             uint32_t ob[8];
 #pragma unroll 1
@@ -595,18 +614,18 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
         const float neg_shift = (shift == neg_inf()) ? 0.f : -shift;
         const uint64_t ns2 = pack2(neg_shift, neg_shift), sc2 = pack2(sc, sc);
-        // (first term, and with kLo the second: what the rounding left)
+        // the first term, and with kLo the second: what the rounding left. The columns of other copies are zeros here.
         auto probabilities = [&](auto lo_tag) {
           constexpr bool kLo = decltype(lo_tag)::value;
-          uint32_t hi[32], lo[kLo ? 32 : 1];
+          uint32_t hi[kCols / 2], lo[kLo ? kCols / 2 : 1];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < kCols / 2; ++e) {
             float x0, x1;
             unpack2(fma2(pack2(__uint_as_float(sr[2 * e]), __uint_as_float(sr[2 * e + 1])), sc2, ns2), x0, x1);
             uint64_t p = pack2(fast_exp2(x0), fast_exp2(x1));
             l2[e & 1] = add2(l2[e & 1], p);
             if constexpr (kQuant) {
-              const ulonglong2 f = ks[TK / 4 + e / 2];
+              const ulonglong2 f = vs[e / 2];
               p = fma2(p, e & 1 ? f.y : f.x, kMinusZero2);
             }
             float p0, p1;
@@ -618,8 +637,20 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               lo[e] = Half16<TP>::down(p0, p1);
             }
           }
-          tmem_st32(tS, hi);
-          if constexpr (kLo) tmem_st32(tS + 32, lo);
+          auto store = [&](uint32_t to, const uint32_t* x) {
+            if constexpr (kCopies == 1) {
+              tmem_st32(to, *reinterpret_cast<const uint32_t(*)[32]>(x));
+            } else {
+              const uint32_t zero[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (i / (kCols / 16) == copy) tmem_st8(to + i * 8, *reinterpret_cast<const uint32_t(*)[8]>(x + i % (kCols / 16) * 8));
+                else tmem_st8(to + i * 8, zero);
+              }
+            }
+          };
+          store(tS, hi);
+          if constexpr (kLo) store(tS + 32, lo);
         };
         if (kMaySplit && split) probabilities(std::integral_constant<bool, kMaySplit>());
         else probabilities(std::integral_constant<bool, false>());
@@ -628,37 +659,49 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
       }
-      ++unit;
-      if (!ok) break;
       // ---- the piece's rows leave ----
-      ok = warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314);
-      if (!ok) break;
+      if (!warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314)) return false;
       tc_fence_after();
       float la, lb, lc, ld;
       unpack2(l2[0], la, lb);
       unpack2(l2[1], lc, ld);
       const float l_run = (la + lb) + (lc + ld);
-      const bool store = row < rows;
-      const float rel = (m_true == neg_inf()) ? 0.f : fast_exp2(shift - m_true);
-      const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0 + row, blockIdx.x);
-      if (store) {
-        // a NaN score passes the maximum by and shows in the sum
-        const float m = (l_run != l_run && m_true < __int_as_float(0x7f800000)) ? l_run : m_true;
-        a.ml[out] = make_float2(m, l_run * rel);
+      float rel = (m_true == neg_inf()) ? 0.f : fast_exp2(shift - m_true);
+      // a NaN score passes the maximum by and shows in the sum
+      float m = (l_run != l_run && m_true < __int_as_float(0x7f800000)) ? l_run : m_true, l = l_run * rel;
+      if constexpr (kCopies > 1) {
+        row_ml[threadIdx.x] = make_float2(m, l);
+        group_sync();
+        float top = neg_inf();
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) top = max_nan(top, row_ml[c * kBlock + row].x);
+        const float ref = top == neg_inf() ? 0.f : top;
+        rel *= fast_exp2(m - ref);
+        l = 0.f;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          const float2 x = row_ml[c * kBlock + row];
+          l += x.y * fast_exp2(x.x - ref);
+        }
+        m = top;
       }
-      float* dst = a.O + out * a.d_pad;
-      constexpr int kA = Widen<TC>::kSwap ? 2 : 1, kB = 3 - kA;  // the columns of 1 and 2
+      const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0, blockIdx.x);
+      if (mine && copy == 0) a.ml[out + row] = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t ob[32];
         tmem_ld32(tO + c * 32, ob);
         tc_wait_ld();
-        if constexpr (kMaySplit && !kQuant) {
-          uint64_t zero[2] = {0ull, 0ull};  // stay 0 while every value is finite
+        [[maybe_unused]] uint64_t zero[2] = {0ull, 0ull};  // stay 0 while every value is finite
+        if constexpr (!kQuant) {
 #pragma unroll
           for (int e = 0; e < 32; e += 2)
             zero[(e >> 1) & 1] = fma2(pack2(__uint_as_float(ob[e]), __uint_as_float(ob[e + 1])), 0ull, zero[(e >> 1) & 1]);
-          if (split && __any_sync(kFullMask, store && ((zero[0] | zero[1]) & 0x7fffffff7fffffffull) != 0ull)) {
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * rel);
+        if constexpr (!kQuant) {
+          if (split && __any_sync(kFullMask, mine && ((zero[0] | zero[1]) & 0x7fffffff7fffffffull) != 0ull)) {
             int32_t first, last, slot, end_slot;
             keys_of(w.t0, first, slot);
             const int left = keys_of(w.t0 + w.n - 1, last, end_slot);
@@ -667,22 +710,45 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               const int f = __shfl_sync(kFullMask, found, e);
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (i == e && f != 0 && l_run == l_run)
-                  ob[i] = f == 2 ? 0x7fc00000u : f > 0 ? 0x7f800000u : 0xff800000u;
+                if (i == e && f != 0 && l == l) ob[i] = f == 2 ? 0x7fc00000u : f > 0 ? 0x7f800000u : 0xff800000u;
             }
           }
         }
-        if (store) {
+        constexpr int kA = Widen<TC>::kSwap ? 2 : 1, kB = 3 - kA;  // the columns of 1 and 2
+        auto four = [&](int e) { return make_uint4(ob[e], ob[e + kA], ob[e + kB], ob[e + 3]); };
+        if constexpr (kCopies == 1) {
+          if (mine) {
+            float* dst = a.O + (out + row) * a.d_pad + c * 32;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 y = make_float4(__uint_as_float(ob[e]) * rel, __uint_as_float(ob[e + kA]) * rel,
-                                         __uint_as_float(ob[e + kB]) * rel, __uint_as_float(ob[e + 3]) * rel);
-            if (c * 32 + e < a.d_pad) *reinterpret_cast<float4*>(dst + c * 32 + e) = y;
+            for (int e = 0; e < 32; e += 4)
+              if (c * 32 + e < a.d_pad) *reinterpret_cast<uint4*>(dst + e) = four(e);
           }
+          __syncwarp();
+        } else {  // the copies are added up where Q was, 32 columns at a time
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + P::unit(threadIdx.x, e / 4)) = four(e);
+          group_sync();
+          for (int x = threadIdx.x; x < rows * 8; x += 128) {
+            const int r = x / 8, u = x % 8;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) {
+              const float4 z = *reinterpret_cast<const float4*>(smem + P::kOffQ + P::unit(k * kBlock + r, u));
+              y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+            }
+            if (c * 32 + u * 4 < a.d_pad) *reinterpret_cast<float4*>(a.O + (out + r) * a.d_pad + c * 32 + u * 4) = y;
+          }
+          group_sync();
         }
-        __syncwarp();
       }
       tc_fence_before();
+      return true;
+    };
+    while (ok && w.next(a)) {
+      const int rows = w.rows(a);
+      if (rows <= 32) ok = piece(std::integral_constant<int, 16>());
+      else if (rows <= 64) ok = piece(std::integral_constant<int, 32>());
+      else ok = piece(std::integral_constant<int, 64>());
     }
   }
 
