@@ -25,7 +25,8 @@ struct e4m3 {
 __device__ __forceinline__ float up1(float x) { return x; }
 __device__ __forceinline__ float up1(__half x) { return __half2float(x); }
 __device__ __forceinline__ float up1(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float up1(int8_t x) { return (float)x; }
+// 8388608 + (code + 128) has the code's bits as its last
+__device__ __forceinline__ float up1(int8_t x) { return __uint_as_float(0x4b000000u | ((uint8_t)x ^ 0x80u)) - 8388736.f; }
 __device__ __forceinline__ float up1(e4m3 x) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)x.bits, __NV_E4M3)));
 }
@@ -33,7 +34,9 @@ __device__ __forceinline__ void down1(float& y, float x) { y = x; }
 __device__ __forceinline__ void down1(__half& y, float x) { y = __float2half_rn(x); }
 __device__ __forceinline__ void down1(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
 // |x| <= 127 (1 + 2^-23) here: row_scale's inverse times an element of its row
-__device__ __forceinline__ void down1(int8_t& y, float x) { y = (int8_t)__float2int_rn(x); }
+// (the sum is rounded to a whole number, to even where it is half way: its last byte is the code; x itself was
+// rounded before)
+__device__ __forceinline__ void down1(int8_t& y, float x) { y = (int8_t)__float_as_uint(__fadd_rn(x, 12582912.f)); }
 __device__ __forceinline__ void down1(e4m3& y, float x) { y.bits = __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
 
 template <class T> struct IsByte { static constexpr bool value = sizeof(T) == 1; };
@@ -67,8 +70,9 @@ __device__ __forceinline__ void load_vec(const T* p, float (&x)[N]) {
     for (int i = 0; i < N; ++i) x[i] = up1(u.e[i]);
   }
 }
+// (all zeros where `none`)
 template <class T, int N>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[N], bool none = false) {
   using Raw = typename RawOf<N * (int)sizeof(T)>::type;
   union {
     Raw raw;
@@ -85,6 +89,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) down1(u.e[i], x[i]);
   }
+  if (none) u.raw = Raw{};
   *reinterpret_cast<Raw*>(p) = u.raw;
 }
 

@@ -14,6 +14,7 @@ struct RowsView {  // rows of a call: [n_rows, heads, d], d contiguous
   int64_t k_stride[2], v_stride[2];  // elements from row to row, head to head
   const int32_t* cu_rows;
   int64_t n_rows;
+  int64_t first;  // of the launch: its group numbers are 32-bit
 };
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -38,53 +39,64 @@ __device__ __forceinline__ Place place_of(const CacheView& c, const int32_t* cu,
 
 constexpr int kThreads = 256;
 
-// One group of LPR lanes per row and head, VE elements of K and of V in each lane: the loads of both are in flight together.
-// d <= VE * LPR, d % VE == 0, every row VE elements aligned (to 16 bytes in the wider of the two types).
-template <class TIn, class TC, int VE, int LPR>
+// Which row and heads a group of lanes works on: rows first, then pieces of `HC` heads.
+template <int LPR, int HC>
+struct Task {
+  uint32_t i;
+  int32_t h0;
+  __device__ __forceinline__ Task(const CacheView& c) {
+    const uint32_t group = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) / LPR, parts = (uint32_t)(c.n_heads + HC - 1) / HC;
+    i = group / parts;
+    h0 = (int32_t)(group - i * parts) * HC;
+  }
+};
+
+// One group of LPR lanes per row and HC heads, VE elements of K and of V of every head in each lane: all loads are in flight
+// together, and the row's place in the cache is found once. d <= VE * LPR, d % VE == 0, every row VE elements aligned (to 16 bytes in
+// the wider of the two types). Bound by the bytes that it reads and writes.
+template <class TIn, class TC, int VE, int LPR, int HC>
 __global__ void __launch_bounds__(kThreads) append_kernel(const RowsView rows, const CacheView c) {
-  const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
+  using Raw = typename RawOf<VE * (int)sizeof(TIn)>::type;
+  const Task<LPR, HC> task(c);
   const int e0 = (threadIdx.x % LPR) * VE;
-  const int64_t i = group / c.n_heads;
-  const int32_t h = (int32_t)(group - i * c.n_heads);
-  const bool some = i < rows.n_rows && e0 < c.d;  // lanes without elements take part in the shuffles
-  float k[VE], v[VE];
+  const int64_t i = rows.first + task.i;
+  const bool row = i < rows.n_rows, some = row && e0 < c.d;  // lanes without elements take part in the shuffles
+  Raw raw[HC][2];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) k[e] = v[e] = 0.f;
-  if (some) {
-    load_vec<TIn, VE>(reinterpret_cast<const TIn*>(rows.K) + i * rows.k_stride[0] + h * rows.k_stride[1] + e0, k);
-    load_vec<TIn, VE>(reinterpret_cast<const TIn*>(rows.V) + i * rows.v_stride[0] + h * rows.v_stride[1] + e0, v);
+  for (int x = 0; x < HC; ++x) {
+    raw[x][0] = raw[x][1] = Raw{};
+    if (some && task.h0 + x < c.n_heads) {
+      const int64_t h = task.h0 + x;
+      raw[x][0] = __ldcs(reinterpret_cast<const Raw*>(reinterpret_cast<const TIn*>(rows.K) + i * rows.k_stride[0] + h * rows.k_stride[1] + e0));
+      raw[x][1] = __ldcs(reinterpret_cast<const Raw*>(reinterpret_cast<const TIn*>(rows.V) + i * rows.v_stride[0] + h * rows.v_stride[1] + e0));
+    }
   }
   Place at = {-1, 0};
-  if (i < rows.n_rows) at = place_of(c, rows.cu_rows, i);
-  float sk = 1.f, sv = 1.f;
-  if constexpr (IsByte<TC>::value) {
-    float tk = 0.f, tv = 0.f;
+  if (row) at = place_of(c, rows.cu_rows, i);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      tk = max_nan(tk, fabsf(k[e]));
-      tv = max_nan(tv, fabsf(v[e]));
-    }
+  for (int x = 0; x < HC; ++x) {
+    const int64_t h = task.h0 + x;
+    const bool here = some && at.page >= 0 && h < c.n_heads;
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) {
-      tk = max_nan(tk, __shfl_xor_sync(0xffffffffu, tk, o));
-      tv = max_nan(tv, __shfl_xor_sync(0xffffffffu, tv, o));
-    }
-    float ik, iv;
-    sk = row_scale<TC>(tk, ik);
-    sv = row_scale<TC>(tv, iv);
+    for (int kv = 0; kv < 2; ++kv) {
+      const Pages& pages = kv ? c.V : c.K;
+      float y[VE];
+      load_vec<TIn, VE>(reinterpret_cast<const TIn*>(&raw[x][kv]), y);
+      bool none = false;
+      if constexpr (IsByte<TC>::value) {
+        float top = 0.f;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      k[e] *= ik;
-      v[e] *= iv;
-    }
-  }
-  if (at.page < 0 || !some) return;
-  store_vec<TC, VE>(reinterpret_cast<TC*>(c.K.data) + c.K.at(at.page, at.slot, h) + e0, k);
-  store_vec<TC, VE>(reinterpret_cast<TC*>(c.V.data) + c.V.at(at.page, at.slot, h) + e0, v);
-  if constexpr (IsByte<TC>::value) {
-    if (e0 == 0) {
-      c.K.scale[c.K.scale_at(at.page, at.slot, h)] = sk;
-      c.V.scale[c.V.scale_at(at.page, at.slot, h)] = sv;
+        for (int e = 0; e < VE; ++e) top = max_nan(top, fabsf(y[e]));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float inverse;
+        const float scale = row_scale<TC>(top, inverse);
+        none = scale != scale;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y[e] *= inverse;
+        if (here && e0 == 0) pages.scale[pages.scale_at(at.page, at.slot, h)] = scale;
+      }
+      if (here) store_vec<TC, VE>(reinterpret_cast<TC*>(pages.data) + pages.at(at.page, at.slot, h) + e0, y, none);
     }
   }
 }
@@ -92,62 +104,80 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const RowsView rows, c
 // Any d, any alignment: one warp per row and head, element by element; the row is read twice where it is quantised.
 template <class TIn, class TC>
 __global__ void __launch_bounds__(kThreads) append_any_kernel(const RowsView rows, const CacheView c) {
-  const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  const uint32_t group = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
-  const int64_t i = group / c.n_heads;
-  const int32_t h = (int32_t)(group - i * c.n_heads);
+  const int64_t i = rows.first + group / c.n_heads;
+  const int32_t h = (int32_t)(group % c.n_heads);
   if (i >= rows.n_rows) return;
   const Place at = place_of(c, rows.cu_rows, i);
   if (at.page < 0) return;
   auto one = [&](const TIn* src, const Pages& pages) {
     float inverse = 1.f;
+    bool none = false;
     if constexpr (IsByte<TC>::value) {
       float top = 0.f;
       for (int e = lane; e < c.d; e += 32) top = max_nan(top, fabsf(up1(src[e])));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float scale = row_scale<TC>(top, inverse);
+      none = scale != scale;
       if (lane == 0) pages.scale[pages.scale_at(at.page, at.slot, h)] = scale;
     }
     TC* dst = reinterpret_cast<TC*>(pages.data) + pages.at(at.page, at.slot, h);
-    for (int e = lane; e < c.d; e += 32) down1(dst[e], up1(src[e]) * inverse);
+    for (int e = lane; e < c.d; e += 32) down1(dst[e], none ? 0.f : up1(src[e]) * inverse);
   };
   one(reinterpret_cast<const TIn*>(rows.K) + i * rows.k_stride[0] + h * rows.k_stride[1], c.K);
   one(reinterpret_cast<const TIn*>(rows.V) + i * rows.v_stride[0] + h * rows.v_stride[1], c.V);
 }
 
 // The way back: x = q * scale in 32 bits, rounded once to the output's type. Same groups of lanes as append_kernel.
-template <class TOut, class TC, int VE, int LPR>
+template <class TOut, class TC, int VE, int LPR, int HC>
 __global__ void __launch_bounds__(kThreads) read_kernel(const RowsView rows, const CacheView c) {
-  const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
+  using Raw = typename RawOf<VE * (int)sizeof(TC)>::type;
+  const Task<LPR, HC> task(c);
   const int e0 = (threadIdx.x % LPR) * VE;
-  const int64_t i = group / c.n_heads;
-  const int32_t h = (int32_t)(group - i * c.n_heads);
+  const int64_t i = rows.first + task.i;
   if (i >= rows.n_rows || e0 >= c.d) return;
   const Place at = place_of(c, rows.cu_rows, i);
   if (at.page < 0) return;
-  float k[VE], v[VE], sk = 1.f, sv = 1.f;
-  load_vec<TC, VE>(reinterpret_cast<const TC*>(c.K.data) + c.K.at(at.page, at.slot, h) + e0, k);
-  load_vec<TC, VE>(reinterpret_cast<const TC*>(c.V.data) + c.V.at(at.page, at.slot, h) + e0, v);
-  if constexpr (IsByte<TC>::value) {
-    sk = c.K.scale[c.K.scale_at(at.page, at.slot, h)];
-    sv = c.V.scale[c.V.scale_at(at.page, at.slot, h)];
+  Raw raw[HC][2];
+  float scale[HC][2];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      k[e] *= sk;
-      v[e] *= sv;
+  for (int x = 0; x < HC; ++x) {
+    const int64_t h = task.h0 + x;
+    if (h >= c.n_heads) continue;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const Pages& pages = kv ? c.V : c.K;
+      raw[x][kv] = *reinterpret_cast<const Raw*>(reinterpret_cast<const TC*>(pages.data) + pages.at(at.page, at.slot, h) + e0);
+      if constexpr (IsByte<TC>::value) scale[x][kv] = pages.scale[pages.scale_at(at.page, at.slot, h)];
     }
   }
-  store_vec<TOut, VE>(reinterpret_cast<TOut*>(rows.K) + i * rows.k_stride[0] + h * rows.k_stride[1] + e0, k);
-  store_vec<TOut, VE>(reinterpret_cast<TOut*>(rows.V) + i * rows.v_stride[0] + h * rows.v_stride[1] + e0, v);
+#pragma unroll
+  for (int x = 0; x < HC; ++x) {
+    const int64_t h = task.h0 + x;
+    if (h >= c.n_heads) continue;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float y[VE];
+      load_vec<TC, VE>(reinterpret_cast<const TC*>(&raw[x][kv]), y);
+      if constexpr (IsByte<TC>::value) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y[e] *= scale[x][kv];
+      }
+      TOut* dst = kv ? reinterpret_cast<TOut*>(rows.V) + i * rows.v_stride[0] + h * rows.v_stride[1]
+                     : reinterpret_cast<TOut*>(rows.K) + i * rows.k_stride[0] + h * rows.k_stride[1];
+      store_vec<TOut, VE>(dst + e0, y);
+    }
+  }
 }
 
 template <class TOut, class TC>
 __global__ void __launch_bounds__(kThreads) read_any_kernel(const RowsView rows, const CacheView c) {
-  const int64_t group = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  const uint32_t group = (blockIdx.x * (uint32_t)kThreads + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
-  const int64_t i = group / c.n_heads;
-  const int32_t h = (int32_t)(group - i * c.n_heads);
+  const int64_t i = rows.first + group / c.n_heads;
+  const int32_t h = (int32_t)(group % c.n_heads);
   if (i >= rows.n_rows) return;
   const Place at = place_of(c, rows.cu_rows, i);
   if (at.page < 0) return;

@@ -13,45 +13,50 @@ int check_rows_arg(const void* K, const int64_t* ks, const void* V, const int64_
   return SPFA_OK;
 }
 
-// One launch over (row, head): `lanes` threads each.
-int grid_of(int64_t n_rows, int64_t heads, int lanes, unsigned& blocks) {
-  const int64_t n = (n_rows * heads * lanes + cache::kThreads - 1) / cache::kThreads;
-  if (n > kMost32) return SPFA_ERR_TOO_LARGE;
-  blocks = (unsigned)n;
-  return SPFA_OK;
+// launch(rows, blocks) for the rows of the call, `lanes` threads for each of a row's `parts`; thread numbers stay below 2^31.
+template <class F>
+int launch_over_rows(cache::RowsView rows, int64_t parts, int lanes, F&& launch) {
+  const int64_t most = (kMost32 - cache::kThreads) / (parts * lanes);
+  for (rows.first = 0; rows.first < rows.n_rows; rows.first += most) {
+    const int64_t n = rows.n_rows - rows.first < most ? rows.n_rows - rows.first : most;
+    launch(rows, (unsigned)((n * parts * lanes + cache::kThreads - 1) / cache::kThreads));
+    g_launches.fetch_add(1);
+  }
+  return launch_status();
 }
+
+// Threads that fill the machine (148 SMs of 2048): from there on a group of lanes takes four heads of its row.
+constexpr int64_t kManyThreads = 148 * 2048;
 
 template <bool kAppend, class T, class TC>
 int launch_rows(const spfa_kv_cache* c, const cache::RowsView& rows, cudaStream_t st) {
   constexpr int VE = 16 / (int)sizeof(T);
   const CacheView view = cache_view(c);
-  unsigned blocks = 0;
-  int rc = SPFA_OK;
   // Pieces of 16 bytes of the rows' type: a row of up to 32 of them stays in its lanes' registers. Others go element by element.
   if (c->d <= VE * 32 && cache_rows_align(c, VE) && rows_align(rows.K, rows.k_stride, sizeof(T), VE) &&
       rows_align(rows.V, rows.v_stride, sizeof(T), VE)) {
-    auto run = [&](auto lanes) {
-      constexpr int LPR = decltype(lanes)::value;
-      rc = grid_of(rows.n_rows, c->n_heads, LPR, blocks);
-      if (rc != SPFA_OK) return;
-      if constexpr (kAppend) cache::append_kernel<T, TC, VE, LPR><<<blocks, cache::kThreads, 0, st>>>(rows, view);
-      else cache::read_kernel<T, TC, VE, LPR><<<blocks, cache::kThreads, 0, st>>>(rows, view);
+    auto run = [&](auto lanes, auto heads) {
+      constexpr int LPR = decltype(lanes)::value, HC = decltype(heads)::value;
+      return launch_over_rows(rows, (c->n_heads + HC - 1) / HC, LPR, [&](const cache::RowsView& r, unsigned blocks) {
+        if constexpr (kAppend) cache::append_kernel<T, TC, VE, LPR, HC><<<blocks, cache::kThreads, 0, st>>>(r, view);
+        else cache::read_kernel<T, TC, VE, LPR, HC><<<blocks, cache::kThreads, 0, st>>>(r, view);
+      });
+    };
+    auto by_heads = [&](auto lanes) {
+      return (c->n_heads > 1 && rows.n_rows * c->n_heads * decltype(lanes)::value > kManyThreads)
+                 ? run(lanes, std::integral_constant<int, 4>())
+                 : run(lanes, std::integral_constant<int, 1>());
     };
     const int need = c->d / VE;
-    if (need <= 4) run(std::integral_constant<int, 4>());
-    else if (need <= 8) run(std::integral_constant<int, 8>());
-    else if (need <= 16) run(std::integral_constant<int, 16>());
-    else run(std::integral_constant<int, 32>());
-  } else {
-    rc = grid_of(rows.n_rows, c->n_heads, 32, blocks);
-    if (rc == SPFA_OK) {
-      if constexpr (kAppend) cache::append_any_kernel<T, TC><<<blocks, cache::kThreads, 0, st>>>(rows, view);
-      else cache::read_any_kernel<T, TC><<<blocks, cache::kThreads, 0, st>>>(rows, view);
-    }
+    if (need <= 4) return by_heads(std::integral_constant<int, 4>());
+    if (need <= 8) return by_heads(std::integral_constant<int, 8>());
+    if (need <= 16) return by_heads(std::integral_constant<int, 16>());
+    return by_heads(std::integral_constant<int, 32>());
   }
-  if (rc != SPFA_OK) return rc;
-  g_launches.fetch_add(1);
-  return launch_status();
+  return launch_over_rows(rows, c->n_heads, 32, [&](const cache::RowsView& r, unsigned blocks) {
+    if constexpr (kAppend) cache::append_any_kernel<T, TC><<<blocks, cache::kThreads, 0, st>>>(r, view);
+    else cache::read_any_kernel<T, TC><<<blocks, cache::kThreads, 0, st>>>(r, view);
+  });
 }
 
 template <bool kAppend>
@@ -61,7 +66,7 @@ int rows_call(const spfa_kv_cache* c, int dtype, void* K, const int64_t* ks, voi
   if (rc == SPFA_OK) rc = check_rows_arg(K, ks, V, vs, cu, n_rows, dtype);
   if (rc != SPFA_OK) return rc;
   if (n_rows == 0 || c->n_seq == 0 || c->n_pages == 0 || c->table_width == 0) return SPFA_OK;
-  cache::RowsView rows{static_cast<char*>(K), static_cast<char*>(V), {ks[0], ks[1]}, {vs[0], vs[1]}, cu, n_rows};
+  cache::RowsView rows{static_cast<char*>(K), static_cast<char*>(V), {ks[0], ks[1]}, {vs[0], vs[1]}, cu, n_rows, 0};
   return with_cache_types(dtype, c->dtype, [&](auto* t, auto* tc) {
     using T = typename std::remove_pointer<decltype(t)>::type;
     using TC = typename std::remove_pointer<decltype(tc)>::type;
