@@ -6,19 +6,20 @@
 namespace spfa {
 namespace {
 
-constexpr int kCtas = 296;  // of the context kernel: two on each of 148 SMs
+constexpr int kCtas = 296;     // of the tensor-core context kernel: two on each of 148 SMs
+constexpr int kAnyCtas = 296;  // of the other one
 
 struct TreeLayout {
-  int row_tile, d_pad;  // row_tile: of the larger units
+  int d_pad;
   int64_t rows;
   size_t cut, ml, O, total;
 };
 TreeLayout tree_layout(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
   TreeLayout t{};
   // either context kernel must fit: which one runs is settled by the call
-  t.row_tile = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? tree::kTiledRows : tree::kAnyRows;
+  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? tree::kTiledRows * kCtas : tree::kAnyRows * kAnyCtas;
   t.d_pad = (c->d + 3) / 4 * 4;
-  t.rows = n_rows * n_q_heads + (int64_t)t.row_tile * kCtas;
+  t.rows = n_rows * n_q_heads + pieces;
   t.cut = 0;
   t.ml = align_up((size_t)(c->n_seq + 1) * 8);
   t.O = t.ml + align_up((size_t)t.rows * 8);
@@ -39,11 +40,22 @@ bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t*
   return dtype == SPFA_DTYPE_F16 ? tree::usable_f16(c) : tree::usable_bf16(c);
 }
 
+// Calls that direct_kernel takes: its CTAs, one on an SM, walk their keys in few rounds. The page lists bound the keys; lens is not
+// known here.
+constexpr double kDirectRounds = 2;
+bool direct_call(const tree::Call& a, const spfa_kv_cache* c, bool vec) {
+  const int size = dtype_bytes(c->dtype);
+  if (!vec || c->d > 128 || !cache_rows_align(c, 16 / size)) return false;
+  const double waves = (double)((a.n_rows * c->n_heads * ((a.group + tree::kDirectRows - 1) / tree::kDirectRows) + 147) / 148);
+  const int keys = tree::DirectPlan(c->d * size).warps * 32;
+  return waves * (double)((a.c.capacity + keys - 1) / keys) <= kDirectRounds;
+}
+
 // One wave of CTAs, or as many as there can be shares of the list: lens is not known here, the page lists bound it.
-int grid_of(const tree::Call& a) {
+int grid_of(const tree::Call& a, int ctas) {
   const double tiles = (double)a.tiles_of(a.c.capacity), rows = (double)a.n_rows * a.group / a.row_tile + a.c.n_seq;
   const double most = tiles * rows * a.c.n_heads / a.least;
-  return most < kCtas ? (most < 1 ? 1 : (int)most) : kCtas;
+  return most < ctas ? (most < 1 ? 1 : (int)most) : ctas;
 }
 
 }  // namespace
@@ -81,7 +93,9 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   a.n_q_heads = (int32_t)n_q_heads;
   a.group = (int32_t)(n_q_heads / c->n_heads);
   a.scale_log2e = (1.0f / sqrtf((float)c->d)) * kLog2e;
-  const bool tiled = g_path.load() != SPFA_PATH_GATHER && tiled_call(c, dtype, Q, Q_stride);
+  const bool vec = cache_rows_align(c, 4) && rows_align(Q, Q_stride, size, 4) && rows_align(O, O_stride, size, 4);
+  a.direct = g_path.load() == SPFA_PATH_AUTO && direct_call(a, c, vec);
+  const bool tiled = g_path.load() != SPFA_PATH_GATHER && !a.direct && tiled_call(c, dtype, Q, Q_stride);
   if (g_path.load() == SPFA_PATH_TILED && !tiled) return SPFA_ERR_BAD_ARG;
   if (tiled) {
     a.row_tile = tree::kTiledRows;
@@ -94,7 +108,7 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
     a.page_tiles = 0;
   }
   a.least = 1;
-  a.n_cta = grid_of(a);
+  a.n_cta = grid_of(a, tiled ? kCtas : kAnyCtas);
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
   a.ml = reinterpret_cast<float2*>(ws + t.ml);
@@ -109,7 +123,6 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   g.o_stride[0] = O_stride[0];
   g.o_stride[1] = O_stride[1];
   g.first = first ? 1 : 0;
-  const bool vec = cache_rows_align(c, 4) && rows_align(Q, Q_stride, size, 4) && rows_align(O, O_stride, size, 4);
   cudaStream_t st = (cudaStream_t)stream;
   g_last_path.store(tiled ? SPFA_PATH_TILED : SPFA_PATH_GATHER);
   if (dtype == SPFA_DTYPE_F16) return tree::launch_f16(c, a, g, vec, tiled, st);

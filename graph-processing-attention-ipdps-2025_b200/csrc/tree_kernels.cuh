@@ -37,6 +37,7 @@ struct Call {
   int32_t page_tiles;           // tiles of a page (pages of tile_keys positions and more), 0: a tile spans whole pages
   int32_t least;                // key tiles that a CTA takes at least
   int32_t n_cta;                // grid of the context kernel
+  int32_t direct;               // the call runs as one launch of direct_kernel
   // workspace
   int64_t* cut;   // [0]: tiles per CTA, [1 + b]: first tile of sequence b in the list
   float2* ml;     // maximum and sum of a piece's row
@@ -425,6 +426,48 @@ struct MergeArgs {
   int first;
 };
 
+// The last of a row (one warp): its keys' maximum M, sum L and un-normalised O meet the incoming state, and the row is stored.
+template <class TQ, int VE, int NC>
+__device__ __forceinline__ void finish_row(const Call& a, const MergeArgs& g, int64_t n, int32_t hq, int lane, float M, float L,
+                                           float (&acc)[NC * VE]) {
+  const int d = a.c.d;
+  auto col = [&](int i) { return (i * 32 + lane) * VE; };
+  float* m = g.m + n * a.n_q_heads + hq;
+  float* l = g.l + n * a.n_q_heads + hq;
+  const bool none = M == neg_inf();  // no key, or none with a score above -inf
+  if (none && !g.first) return;
+  TQ* O = reinterpret_cast<TQ*>(g.O) + n * g.o_stride[0] + hq * g.o_stride[1];
+  float m_out = M * 0.6931471805599453f, keep = 0.f, mine = 1.f;
+  if (!g.first) {
+    const float m_in = *m, l_in = *l;
+    if (l_in != 0.f) {  // a row with l = 0 is empty: what its O holds does not count
+      const float m2 = m_in * kLog2e, top = max_nan(m2, M);
+      if (!(M > m2)) m_out = top != top ? top : m_in;
+      mine = fast_exp2(M - top);
+      keep = l_in * fast_exp2(m2 - top);
+      L = fmaf(L, mine, keep);
+    }
+  }
+  const float inv = none ? 0.f : 1.f / L;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (col(i) < d) {
+      float y[VE];
+      if (keep != 0.f) load_vec<TQ, VE>(O + col(i), y);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float x = acc[i * VE + e] * mine;
+        y[e] = (keep != 0.f ? fmaf(keep, y[e], x) : x) * inv;
+      }
+      store_vec<TQ, VE>(O + col(i), y);
+    }
+  __syncwarp();
+  if (lane == 0) {
+    *m = m_out;
+    *l = none ? 0.f : L;
+  }
+}
+
 template <class TQ, class TC, int VE, int NC>
 __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArgs g) {
   const int lane = threadIdx.x & 31;
@@ -564,40 +607,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArg
     }
   }
 
-  float* m = g.m + n * a.n_q_heads + hq;
-  float* l = g.l + n * a.n_q_heads + hq;
-  const bool none = M == neg_inf();  // no key, or none with a score above -inf
-  if (none && !g.first) return;
-  TQ* O = reinterpret_cast<TQ*>(g.O) + n * g.o_stride[0] + hq * g.o_stride[1];
-  float m_out = M * 0.6931471805599453f, keep = 0.f, mine = 1.f;
-  if (!g.first) {
-    const float m_in = *m, l_in = *l;
-    if (l_in != 0.f) {  // a row with l = 0 is empty: what its O holds does not count
-      const float m2 = m_in * kLog2e, top = max_nan(m2, M);
-      if (!(M > m2)) m_out = top != top ? top : m_in;
-      mine = fast_exp2(M - top);
-      keep = l_in * fast_exp2(m2 - top);
-      L = fmaf(L, mine, keep);
-    }
-  }
-  const float inv = none ? 0.f : 1.f / L;
-#pragma unroll
-  for (int i = 0; i < NC; ++i)
-    if (col(i) < d) {
-      float y[VE];
-      if (keep != 0.f) load_vec<TQ, VE>(O + col(i), y);
-#pragma unroll
-      for (int e = 0; e < VE; ++e) {
-        const float x = acc[i * VE + e] * mine;
-        y[e] = (keep != 0.f ? fmaf(keep, y[e], x) : x) * inv;
-      }
-      store_vec<TQ, VE>(O + col(i), y);
-    }
-  __syncwarp();
-  if (lane == 0) {
-    *m = m_out;
-    *l = none ? 0.f : L;
-  }
+  finish_row<TQ, VE, NC>(a, g, n, hq, lane, M, L, acc);
 }
 
 }  // namespace tree

@@ -2,6 +2,7 @@
 #pragma once
 #include "cache_view.cuh"
 #include "tensor_map.cuh"
+#include "tree_direct.cuh"
 #include "tree_kernels.cuh"
 #include "tree_tiled.cuh"
 
@@ -73,9 +74,27 @@ int launch_merge_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t s
   return launch_merge<TQ, TC, 1, 32>(a, g, st);
 }
 
+template <class TQ, class TC, int R>
+int launch_direct_rows(const Call& a, const MergeArgs& g, cudaStream_t st) {
+  const DirectPlan plan(a.c.d * (int)sizeof(TC));
+  if (!opt_in<direct_kernel<TQ, TC, R>>(227 * 1024)) return SPFA_ERR_LAUNCH;
+  const int64_t blocks = a.n_rows * a.c.n_heads * ((a.group + R - 1) / R);
+  direct_kernel<TQ, TC, R><<<(unsigned)blocks, plan.warps * 32, plan.bytes, st>>>(a, g);
+  g_launches.fetch_add(1);
+  return launch_status();
+}
+template <class TQ, class TC>
+int launch_direct(const Call& a, const MergeArgs& g, cudaStream_t st) {
+  if (a.group == 1) return launch_direct_rows<TQ, TC, 1>(a, g, st);
+  if (a.group == 2) return launch_direct_rows<TQ, TC, 2>(a, g, st);
+  if (a.group <= 4) return launch_direct_rows<TQ, TC, 4>(a, g, st);
+  return launch_direct_rows<TQ, TC, kDirectRows>(a, g, st);
+}
+
 template <class TQ, class TC>
 int launch_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
   const int d = a.c.d;
+  if (a.direct) return launch_direct<TQ, TC>(a, g, st);
   int rc = SPFA_OK;
   if (d <= 64) rc = launch_context_any<64, TQ, TC>(a, vec, st);
   else if (d <= 128) rc = launch_context_any<128, TQ, TC>(a, vec, st);

@@ -485,7 +485,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             if ((u0 + i) * 8 < a.c.d) q[i] = __ldg(reinterpret_cast<const uint4*>(src) + u0 + i);
           }
         };
-        float f = 1.f;
+        [[maybe_unused]] float f = 1.f;
         if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {  // times 2^(14 - exponent of the row's largest element)
           uint32_t top = 0;
 #pragma unroll 1

@@ -58,14 +58,20 @@ def run(pkg, c, Q, cu, mask, state=None):
 
 
 def both_paths(pkg, *args, **kw):
-    """The automatic choice, and the kernel without tensor cores where the choice was another."""
+    """The automatic choice (small calls: one launch), the tensor cores where they can take the call, and the kernels without."""
     yield "auto", run(pkg, *args, **kw)
-    if pkg.capi.last_path() == pkg.capi.PATH_TILED:
-        pkg.capi.set_path(pkg.capi.PATH_GATHER)
+    for tag, path in (("tiled", pkg.capi.PATH_TILED), ("gather", pkg.capi.PATH_GATHER)):
+        pkg.capi.set_path(path)
         try:
-            yield "gather", run(pkg, *args, **kw)
+            try:
+                got = run(pkg, *args, **kw)
+            except RuntimeError as e:
+                assert path == pkg.capi.PATH_TILED and "bad argument" in str(e)
+                continue
+            assert pkg.capi.last_path() == path
         finally:
             pkg.capi.set_path(pkg.capi.PATH_AUTO)
+        yield tag, got
 
 
 SHAPES = [  # lens, rows, Hq, Hkv, d, page, layout
@@ -107,7 +113,7 @@ def test_state_chains(pkg, dtype, cache):
     c2, _, _, mask2 = problem(dtype, cache, [77, 0, 130], [4, 6, 2], 4, 2, 64, 32, seed=6)
     mask2[5] = False
     one, b1, written = tree_reference(c1, Q, cu, mask)
-    for path in (pkg.capi.PATH_AUTO, pkg.capi.PATH_GATHER):
+    for path in (pkg.capi.PATH_AUTO, pkg.capi.PATH_GATHER) + ((pkg.capi.PATH_TILED,) if dtype != "f32" else ()):
         pkg.capi.set_path(path)
         try:
             state = run(pkg, c1, Q, cu, mask)
@@ -377,7 +383,7 @@ def test_which_kernel_takes_a_call(pkg):
                                                ("bf16", "native", 64, 16, 1, False), ("f32", "int8", 64, 16, 0, False)):
         c, Q, cu, mask = problem(dtype, cache, [70], [2], 2, 1, d, page, shift=shift)
         run(pkg, c, Q, cu, mask)
-        assert (pkg.capi.last_path() == tiled) == want, (dtype, cache, d, page, shift)
+        assert pkg.capi.last_path() == pkg.capi.PATH_GATHER  # small: one launch, or the kernels without tensor cores
         pkg.capi.set_path(tiled)
         try:
             if want:
@@ -387,6 +393,9 @@ def test_which_kernel_takes_a_call(pkg):
                     run(pkg, c, Q, cu, mask)
         finally:
             pkg.capi.set_path(pkg.capi.PATH_AUTO)
+        c, Q, cu, mask = problem(dtype, cache, [2048], [150], 2, 1, d, page, shift=shift)
+        run(pkg, c, Q, cu, mask)
+        assert (pkg.capi.last_path() == tiled) == want, (dtype, cache, d, page, shift)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
