@@ -74,11 +74,12 @@ def _check_band_kernel_registers(ptxas_log: str) -> None:
                          ptxas_log, flags=re.S):
         if int(m.group(2)) != 128:
             raise RuntimeError(f"{m.group(1)}: ptxas assigned {m.group(2)} registers, the setmaxnreg budgets need 128")
+    # <padded d, type of Q, type of the cache, row tiles of a CTA>; an 8-bit cache's kernel has more warps
     for m in re.finditer(r"Compiling entry function '(_ZN4spfa4tree20context_tiled_kernelILi\d+E(6__halfS2_|13__nv_bfloat16S2_)?"
-                         r"[^']*)'.*?Used (\d+) registers", ptxas_log, flags=re.S):
-        need = 128 if m.group(2) else 80  # an 8-bit cache's kernel has four warps more
-        if int(m.group(3)) != need:
-            raise RuntimeError(f"{m.group(1)}: ptxas assigned {m.group(3)} registers, the setmaxnreg budgets need {need}")
+                         r"[^']*?Li(\d)EEv[^']*)'.*?Used (\d+) registers", ptxas_log, flags=re.S):
+        need = {"1": (80, 128), "2": (96, 168)}[m.group(3)][1 if m.group(2) else 0]
+        if int(m.group(4)) != need:
+            raise RuntimeError(f"{m.group(1)}: ptxas assigned {m.group(4)} registers, the setmaxnreg budgets need {need}")
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> str:

@@ -7,7 +7,7 @@ namespace spfa {
 namespace {
 
 constexpr int kCtas = 296;     // of the tensor-core context kernel: two on each of 148 SMs
-constexpr int kAnyCtas = 296;  // of the other one
+constexpr int kAnyCtas = 592;  // of the other one where d <= 64, and half as many above
 
 struct TreeLayout {
   int d_pad;
@@ -17,7 +17,7 @@ struct TreeLayout {
 TreeLayout tree_layout(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
   TreeLayout t{};
   // either context kernel must fit: which one runs is settled by the call
-  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? tree::kTiledRows * kCtas : tree::kAnyRows * kAnyCtas;
+  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? 128 * kCtas : tree::kAnyRows * kAnyCtas;
   t.d_pad = (c->d + 3) / 4 * 4;
   t.rows = n_rows * n_q_heads + pieces;
   t.cut = 0;
@@ -35,9 +35,12 @@ int check_tree(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_he
   return SPFA_OK;
 }
 
-bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride) {
+// Row tiles that a CTA of the tensor-core kernel takes together: two where a sequence has more rows than one holds, on average.
+int row_tiles_of(const tree::Call& a) { return a.n_rows * a.group > 128LL * a.c.n_seq ? 2 : 1; }
+
+bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride, int subs) {
   if (dtype == SPFA_DTYPE_F32 || !tree::tiled_shape(c) || !rows_align(Q, Q_stride, 2, 8)) return false;
-  return dtype == SPFA_DTYPE_F16 ? tree::usable_f16(c) : tree::usable_bf16(c);
+  return dtype == SPFA_DTYPE_F16 ? tree::usable_f16(c, subs) : tree::usable_bf16(c, subs);
 }
 
 // Calls that direct_kernel takes: its CTAs, one on an SM, walk their keys in few rounds. The page lists bound the keys; lens is not
@@ -94,11 +97,12 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   a.group = (int32_t)(n_q_heads / c->n_heads);
   a.scale_log2e = (1.0f / sqrtf((float)c->d)) * kLog2e;
   const bool vec = cache_rows_align(c, 4) && rows_align(Q, Q_stride, size, 4) && rows_align(O, O_stride, size, 4);
+  const int subs = row_tiles_of(a);
   a.direct = g_path.load() == SPFA_PATH_AUTO && direct_call(a, c, vec);
-  const bool tiled = g_path.load() != SPFA_PATH_GATHER && !a.direct && tiled_call(c, dtype, Q, Q_stride);
+  const bool tiled = g_path.load() != SPFA_PATH_GATHER && !a.direct && tiled_call(c, dtype, Q, Q_stride, subs);
   if (g_path.load() == SPFA_PATH_TILED && !tiled) return SPFA_ERR_BAD_ARG;
   if (tiled) {
-    a.row_tile = tree::kTiledRows;
+    a.row_tile = 128 * subs;
     const int ps = a.c.page_size, keys = tree::kTiledKeys;
     a.page_tiles = ps >= keys ? (ps + keys - 1) / keys : 0;
     a.tile_keys = ps >= keys ? keys : keys / ps * ps;
@@ -108,7 +112,7 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
     a.page_tiles = 0;
   }
   a.least = 1;
-  a.n_cta = grid_of(a, tiled ? kCtas : kAnyCtas);
+  a.n_cta = grid_of(a, tiled ? kCtas / subs : c->d <= 64 ? kAnyCtas : kAnyCtas / 2);
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
   a.ml = reinterpret_cast<float2*>(ws + t.ml);

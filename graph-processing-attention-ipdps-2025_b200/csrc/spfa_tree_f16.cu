@@ -8,7 +8,7 @@ int launch_f16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool v
   return tiled ? launch_tiled<__half>(c, a, g, vec, st) : launch_by_cache<__half>(c, a, g, vec, st);
 }
 
-bool usable_f16(const spfa_kv_cache* c) { return usable_by_cache<__half>(c); }
+bool usable_f16(const spfa_kv_cache* c, int subs) { return usable_by_cache<__half>(c, subs); }
 
 }  // namespace tree
 }  // namespace spfa

@@ -184,6 +184,9 @@ struct Walk {
 template <int DP>
 struct PlanAny {
   static constexpr int kThreads = 256, kRows = 16;
+  // A tile is a chain of short phases between barriers, and other CTAs fill the gaps: as many as shared memory takes (four where
+  // d <= 64: 16 x 8 heads over 4096 float32 keys in 25 us, with two in 37).
+  static constexpr int kCtasPerSm = DP == 64 ? 4 : DP <= 256 ? 2 : 1;
   static constexpr int TK = DP <= 128 ? 64 : (DP == 256 ? 32 : 16);
   static constexpr int KB = TK / 16, DS = 8 / KB;  // key blocks x slices of d = 8 warps
   static constexpr int CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (4 * CGT);
@@ -195,7 +198,7 @@ struct PlanAny {
 };
 
 template <int DP, class TQ, class TC>
-__global__ void __launch_bounds__(256) context_any_kernel(const Call a, const int vec) {
+__global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kernel(const Call a, const int vec) {
   using P = PlanAny<DP>;
   constexpr int TK = P::TK, R = P::kRows, PITCH = P::kPitch;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -248,11 +251,17 @@ __global__ void __launch_bounds__(256) context_any_kernel(const Call a, const in
         for (int i = 0; i < 4; ++i) o[r][g][i] = 0.f;
     const int rg = tid & 3, cg = (tid >> 2) % P::CGT, ks = tid / (4 * P::CGT);
 
+    auto page_at = [&](int32_t t) -> int32_t {  // of this thread's key of tile t: looked up a tile ahead
+      const int64_t p = (int64_t)t * TK + tid;
+      return tid < TK && t < w.t0 + w.n && p < w.len ? a.c.page_of(w.b, p) : -1;
+    };
+    int32_t next_page = page_at(w.t0);
     for (int32_t t = w.t0; t < w.t0 + w.n; ++t) {
       __syncthreads();  // the last tile's K, V and P are done with
+      const int32_t page = next_page;
+      next_page = page_at(t + 1);
       if (tid < TK) {
         const int64_t p = (int64_t)t * TK + tid;
-        const int32_t page = p < w.len ? a.c.page_of(w.b, p) : -1;
         k_at[tid] = -1;
         if (page >= 0) {
           const int32_t slot = a.c.slot_of(p);

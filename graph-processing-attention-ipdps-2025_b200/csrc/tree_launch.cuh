@@ -14,10 +14,10 @@ namespace tree {
 int launch_f32(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st);
 int launch_f16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, bool tiled, cudaStream_t st);
 int launch_bf16(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, bool tiled, cudaStream_t st);
-bool usable_f16(const spfa_kv_cache* c);
-bool usable_bf16(const spfa_kv_cache* c);
+bool usable_f16(const spfa_kv_cache* c, int subs);
+bool usable_bf16(const spfa_kv_cache* c, int subs);
 
-constexpr int kTiledRows = 128, kTiledKeys = 64;  // unit and tile of context_tiled_kernel
+constexpr int kTiledKeys = 64;  // a tile of context_tiled_kernel
 
 constexpr int kAnyRows = 16;  // row tile of context_any_kernel
 inline int any_tile_keys(int d) { return d <= 128 ? 64 : (d <= 256 ? 32 : 16); }
@@ -134,16 +134,16 @@ bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const in
 }
 
 // As band16_usable: setmaxnreg.inc must be covered by what the launch allocates.
-template <int DP, class T, class TC>
+template <int DP, class T, class TC, int NSUB>
 bool tiled_usable() {
-  using P = PlanTree<DP, TC>;
+  using P = PlanTree<DP, TC, NSUB>;
   static std::atomic<int> cached[64];  // per device: 0 unknown, 1 usable, 2 not
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   int v = cached[dev].load(std::memory_order_relaxed);
   if (v == 0) {
     cudaFuncAttributes attr;
-    auto kern = context_tiled_kernel<DP, T, TC>;
+    auto kern = context_tiled_kernel<DP, T, TC, NSUB>;
     const bool ok = cudaFuncGetAttributes(&attr, kern) == cudaSuccess &&
                     attr.numRegs * P::kThreads >= P::kRegsNeeded &&
                     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kDynSmem) == cudaSuccess;
@@ -153,11 +153,14 @@ bool tiled_usable() {
   return v == 1;
 }
 
-// f(tag of the cache's type, padded d)
+// f(tag of the cache's type, padded d, row tiles of a CTA)
 template <class TQ, class F>
-auto with_tiled(const spfa_kv_cache* c, F&& f) {
+auto with_tiled(const spfa_kv_cache* c, int subs, F&& f) {
+  auto by_subs = [&](auto* t, auto dp) {
+    return subs == 1 ? f(t, dp, std::integral_constant<int, 1>()) : f(t, dp, std::integral_constant<int, 2>());
+  };
   auto by_d = [&](auto* t) {
-    return c->d <= 64 ? f(t, std::integral_constant<int, 64>()) : f(t, std::integral_constant<int, 128>());
+    return c->d <= 64 ? by_subs(t, std::integral_constant<int, 64>()) : by_subs(t, std::integral_constant<int, 128>());
   };
   if (c->dtype == SPFA_DTYPE_E4M3) return by_d(static_cast<e4m3*>(nullptr));
   if (c->dtype == SPFA_DTYPE_INT8) return by_d(static_cast<int8_t*>(nullptr));
@@ -165,23 +168,23 @@ auto with_tiled(const spfa_kv_cache* c, F&& f) {
 }
 
 template <class TQ>
-bool usable_by_cache(const spfa_kv_cache* c) {
-  return with_tiled<TQ>(c, [](auto* t, auto dp) {
-    return tiled_usable<decltype(dp)::value, TQ, typename std::remove_pointer<decltype(t)>::type>();
+bool usable_by_cache(const spfa_kv_cache* c, int subs) {
+  return with_tiled<TQ>(c, subs, [](auto* t, auto dp, auto n) {
+    return tiled_usable<decltype(dp)::value, TQ, typename std::remove_pointer<decltype(t)>::type, decltype(n)::value>();
   });
 }
 
 template <class TQ>
 int launch_tiled(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
-  return with_tiled<TQ>(c, [&](auto* t, auto dp) -> int {
+  return with_tiled<TQ>(c, a.row_tile / 128, [&](auto* t, auto dp, auto n) -> int {
     using TC = typename std::remove_pointer<decltype(t)>::type;
-    constexpr int DP = decltype(dp)::value;
-    using P = PlanTree<DP, TC>;
+    constexpr int DP = decltype(dp)::value, NSUB = decltype(n)::value;
+    using P = PlanTree<DP, TC, NSUB>;
     int* err = tile_error_word();
     CUtensorMap tmK, tmV;
     if (!err || !make_page_map<TC>(&tmK, c, c->K, c->K_stride, DP) || !make_page_map<TC>(&tmV, c, c->V, c->V_stride, DP))
       return SPFA_ERR_LAUNCH;
-    context_tiled_kernel<DP, TQ, TC><<<(unsigned)a.n_cta, P::kThreads, P::kDynSmem, st>>>(tmK, tmV, a, err);
+    context_tiled_kernel<DP, TQ, TC, NSUB><<<(unsigned)a.n_cta, P::kThreads, P::kDynSmem, st>>>(tmK, tmV, a, err);
     g_launches.fetch_add(1);
     const int rc = launch_status();
     return rc != SPFA_OK ? rc : launch_merge_any<TQ, TC>(a, g, vec, st);

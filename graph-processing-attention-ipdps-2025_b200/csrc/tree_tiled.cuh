@@ -31,31 +31,37 @@ namespace tree {
 
 using namespace tile;
 
-template <int DP, class TC>
+// NSUB: 128-row tiles that a CTA works on together, against the same K and V. One, and two CTAs share an SM; or two, and a CTA has it
+// alone: K and V are fetched and converted once for both.
+template <int DP, class TC, int NSUB>
 struct PlanTree {
   static constexpr bool kQuant = sizeof(TC) == 1;
-  static constexpr int kThreads = kQuant ? 384 : 256, kRegsLaunch = kQuant ? 80 : 128;
-  static constexpr int kRegsSoftmax = kQuant ? 128 : 168, kRegsAux = kQuant ? 56 : 88, kConvert = 128;
-  static constexpr int kRegsNeeded = kRegsSoftmax * 128 + kRegsAux * (kThreads - 128);
+  static constexpr int kSoftmaxWarps = 4 * NSUB, kAux = 4 * NSUB /* first of four warps */, kConvertFrom = kAux + 4;
+  static constexpr int kConvert = kQuant ? 128 * NSUB : 0, kThreads = 128 * NSUB + 128 + kConvert, kCtasPerSm = 3 - NSUB;
+  static constexpr int kRegsLaunch = NSUB == 1 ? (kQuant ? 80 : 128) : (kQuant ? 96 : 168);
+  static constexpr int kRegsSoftmax = NSUB == 1 ? (kQuant ? 128 : 168) : (kQuant ? 152 : 184);
+  static constexpr int kRegsAux = NSUB == 1 ? (kQuant ? 56 : 88) : (kQuant ? 56 : 136);
+  static constexpr int kRegsNeeded = kRegsSoftmax * 128 * NSUB + kRegsAux * (kThreads - 128 * NSUB);
   static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
-  static constexpr int TK = 64, kRows = 128, kChunks = DP / 64;
-  static constexpr int kQChunk = kRows * 128, kKVChunk = TK * 128, kQBytes = kChunks * kQChunk;
+  static constexpr int TK = 64, kRows = 128 * NSUB, kChunks = DP / 64;
+  static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128, kQSub = kChunks * kQChunk, kQBytes = NSUB * kQSub;
   static constexpr int kTile = kChunks * kKVChunk;               // a 16-bit tile of K or V
   static constexpr int kStage = kQuant ? TK * DP : kTile;        // a tile as it is fetched
-  static constexpr int NS = DP == 128 ? 2 : 4;                   // stages of K and of V
+  static constexpr int NS = (DP == 128 && NSUB == 1) ? 2 : 4;    // stages of K and of V
+  static constexpr int NC = kQuant ? NSUB : 1;                   // converted tiles of K and of V
   static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
   static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStage, kOffCK = kOffV + NS * kStage;
-  static constexpr int kOffCV = kOffCK + (kQuant ? kTile : 0), kOffScale = kOffCV + (kQuant ? kTile : 0);
-  static constexpr int kOffRow = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffRow + kRows * 8;
-  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 1 + 4 * NS + 4 + 6;
+  static constexpr int kOffCV = kOffCK + (kQuant ? NC * kTile : 0), kOffScale = kOffCV + (kQuant ? NC * kTile : 0);
+  static constexpr int kOffRow = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffRow + 128 * 8;
+  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 4 * NS + 4 * NC + 7 * NSUB;
   static constexpr int kOffCut = kOffBar + kNumBars * 8, kOffMisc = kOffCut + (int)sizeof(Cut);
   static constexpr int kDynSmem = kOffMisc + 16 + 1024;
-  static_assert(2 * (kDynSmem + 1024) <= 228 * 1024, "two CTAs share an SM");
+  static_assert(kCtasPerSm * (kDynSmem + 1024) <= 228 * 1024, "shared memory of an SM");
   // The producer writes the ring's entry of a tile once the tile NS before has left its stage, which is behind the softmax of the
-  // tile two (8-bit: three) before that one.
-  static_assert(NS + 3 <= kRing, "ring entries are written again only after they were read");
-  static constexpr int kColS = 0, kColO = 2 * TK, kTmemCols = 256;
-  static_assert(kColO + DP <= kTmemCols, "S buffers and the O accumulator exceed the TMEM allocation");
+  // tile two (8-bit: two and NC) before that one.
+  static_assert(NS + 2 + NC <= kRing, "ring entries are written again only after they were read");
+  static constexpr int kColS = 0, kColO = NSUB * 2 * TK, kTmemCols = 256 * NSUB;
+  static_assert(kColO + NSUB * DP <= kTmemCols, "S buffers and the O accumulators exceed the TMEM allocation");
   static __device__ __forceinline__ uint32_t unit(int row, int u) { return (uint32_t)(row * 128 + ((u ^ (row & 7)) << 4)); }
 };
 
@@ -155,12 +161,12 @@ __device__ __noinline__ int infinity_of(const Call& a, int32_t b, int32_t h, int
   return (nan || (up && down)) ? 2 : up ? 1 : down ? -1 : 0;
 }
 
-template <int DP, class T, class TC>
-__global__ void __launch_bounds__(PlanTree<DP, TC>::kThreads, 2)
+template <int DP, class T, class TC, int NSUB>
+__global__ void __launch_bounds__(PlanTree<DP, TC, NSUB>::kThreads, PlanTree<DP, TC, NSUB>::kCtasPerSm)
 context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Call a,
                      int* __restrict__ err) {
-  using P = PlanTree<DP, TC>;
-  constexpr int TK = P::TK, NS = P::NS;
+  using P = PlanTree<DP, TC, NSUB>;
+  constexpr int TK = P::TK, NS = P::NS, NC = P::NC;
   constexpr bool kQuant = P::kQuant;
   using TP = typename std::conditional<kQuant, __half, T>::type;  // operands of both products
   constexpr bool kMaySplit = !(kQuant && std::is_same<T, __nv_bfloat16>::value);
@@ -168,8 +174,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + P::kOffBar + 8u * i; };
-  constexpr int B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 1 + NS, B_VFULL = 1 + 2 * NS, B_VEMPTY = 1 + 3 * NS,
-                B_CK = 1 + 4 * NS /* full, empty */, B_CV = B_CK + 2, B_SREADY = B_CK + 4, B_PREADY = B_SREADY + 2, B_OREADY = B_SREADY + 4;
+  constexpr int B_KFULL = 0, B_KEMPTY = NS, B_VFULL = 2 * NS, B_VEMPTY = 3 * NS, B_CK = 4 * NS /* full [NC], empty [NC] */, B_CV = B_CK + 2 * NC, B_SREADY = B_CK + 4 * NC,
+                B_PREADY = B_SREADY + 2 * NSUB, B_OREADY = B_SREADY + 4 * NSUB /* [sub][buffer] */, B_QFULL = B_SREADY + 6 * NSUB;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::kOffMisc + 4);
   Cut* cut = reinterpret_cast<Cut*>(smem + P::kOffCut);
   uint64_t* ring_mask = reinterpret_cast<uint64_t*>(smem + P::kOffMask);
@@ -180,28 +186,32 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   const int n_pages_tile = a.page_tiles ? 1 : a.tile_keys / ps;  // pages of a tile
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(B_QFULL), 128);
     for (int s = 0; s < NS; ++s) {
       mbar_init(bar(B_KFULL + s), kQuant ? 33 : 1);
-      mbar_init(bar(B_KEMPTY + s), kQuant ? 128 : 1);
+      mbar_init(bar(B_KEMPTY + s), kQuant ? P::kConvert / 32 : 1);
       mbar_init(bar(B_VFULL + s), 1);
-      mbar_init(bar(B_VEMPTY + s), kQuant ? 128 : 1);
+      mbar_init(bar(B_VEMPTY + s), kQuant ? P::kConvert / 32 : 1);
     }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(bar(B_CK + 2 * x), 128);
-      mbar_init(bar(B_CK + 2 * x + 1), 1);
+    for (int x = 0; x < NC; ++x) {
+      mbar_init(bar(B_CK + x), kQuant ? P::kConvert / 32 : 1);
+      mbar_init(bar(B_CK + NC + x), 1);
+      mbar_init(bar(B_CV + x), kQuant ? P::kConvert / 32 : 1);
+      mbar_init(bar(B_CV + NC + x), 1);
+    }
+    for (int x = 0; x < 2 * NSUB; ++x) {
       mbar_init(bar(B_SREADY + x), 1);
       mbar_init(bar(B_PREADY + x), 4);
       mbar_init(bar(B_OREADY + x), 1);
     }
+    for (int x = 0; x < NSUB; ++x) mbar_init(bar(B_QFULL + x), 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) {
+  if (warp == P::kAux) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + P::kOffMisc), "r"(P::kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x == 160) {
+  if (threadIdx.x == P::kAux * 32 + 32) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmK)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
   }
@@ -233,11 +243,11 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     return min(left, a.tile_keys);
   };
 
-  if (warp >= 4) {
+  if (warp >= P::kAux) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P::kRegsAux));
-    if (warp == 4 || warp == 6) {
-      // =============================== TMA producers: warp 4 K, masks and scales, warp 6 V ===============================
-      const bool is_k = warp == 4;
+    if (warp == P::kAux || warp == P::kAux + 2) {
+      // =============================== TMA producers: one warp K, masks and scales, one V ===============================
+      const bool is_k = warp == P::kAux;
       const CUtensorMap* tm = is_k ? &tmK : &tmV;
       const int full = is_k ? B_KFULL : B_VFULL, empty = is_k ? B_KEMPTY : B_VEMPTY, off = is_k ? P::kOffK : P::kOffV;
       const bool el = elect_one();
@@ -328,47 +338,58 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
       }
       if constexpr (kQuant) asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == 5) {
+    } else if (warp == P::kAux + 1) {
       // =============================== MMA issuer ===============================
       const bool el = elect_one();
       auto wait = [&](int b, uint32_t parity, int code) -> bool { return warp_wait(bar(b), parity, abort_flag, err, code); };
       constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
       const uint64_t qd = smem_desc(sbase + P::kOffQ, 16, 1024, kLayoutSw128);
-      uint32_t jj = 0, unit = 0;
+      uint32_t jj = 0;
+      uint32_t done[NSUB] = {}, units[NSUB] = {};  // tiles and units of each row tile: an empty second one does not count
       bool ok = true;
       while (ok && w.next(a)) {
         const int32_t n = w.n;
-        const bool split = w.tokens * a.group <= P::kRows;
-        ok = wait(B_QFULL, unit & 1, 211);
-        ++unit;
+        const bool split = w.tokens * a.group <= 128;
+        const int subs = NSUB == 1 ? 1 : (w.rows(a) > 128 ? 2 : 1);
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+          if (sub < subs && ok) ok = warp_wait(bar(B_QFULL + sub), units[sub]++ & 1, abort_flag, err, 211);
         if (!ok) break;
-        auto issue_S = [&](int32_t t) -> bool {
-          if (t >= n) return true;
+        auto k_ready = [&](int32_t t) -> bool {
           const uint32_t j = jj + (uint32_t)t;
-          const int st = kQuant ? 0 : j % NS;
-          if (!wait(kQuant ? B_CK : B_KFULL + st, kQuant ? (j & 1) : ((j / NS) & 1), 212)) return false;
+          return t >= n || warp_wait(bar(kQuant ? B_CK + j % NC : B_KFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 212);
+        };
+        auto issue_S = [&](int32_t t, int sub) {
+          if (t >= n) return;
+          const uint32_t j = jj + (uint32_t)t, buf = (done[sub] + (uint32_t)t) & 1;
+          const int st = kQuant ? j % NC : j % NS;
           tc_fence_after();
-          const uint64_t kd = smem_desc(sbase + (kQuant ? P::kOffCK : P::kOffK + st * P::kStage), 16, 1024, kLayoutSw128);
+          const uint64_t kd = smem_desc(sbase + (kQuant ? P::kOffCK + st * P::kTile : P::kOffK + st * P::kStage), 16, 1024, kLayoutSw128);
           if (el) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {  // 16 elements (32 bytes) of the contraction per MMA
               const int c = kk / 4, in = kk % 4 * 32;
-              mma16_ss(tmem + P::kColS + TK * (j & 1), qd + (uint64_t)((c * P::kQChunk + in) >> 4),
+              mma16_ss(tmem + P::kColS + TK * (2 * sub + buf), qd + (uint64_t)((sub * P::kQSub + c * P::kQChunk + in) >> 4),
                        kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS, kk ? 1u : 0u);
             }
-            tc_commit(bar(B_SREADY + (j & 1)));
-            tc_commit(bar(kQuant ? B_CK + 1 : B_KEMPTY + st));
+            tc_commit(bar(B_SREADY + 2 * sub + buf));
+            if (sub == subs - 1) tc_commit(bar(kQuant ? B_CK + NC + st : B_KEMPTY + st));
           }
           __syncwarp();
-          return true;
         };
-        ok = issue_S(0) && issue_S(1);
+        for (int32_t t = 0; t < 2 && ok; ++t) {
+          ok = k_ready(t);
+          if (!ok) break;
+#pragma unroll
+          for (int sub = 0; sub < NSUB; ++sub)
+            if (sub < subs) issue_S(t, sub);
+        }
         for (int32_t t = 0; t < n && ok; ++t) {
           const uint32_t j = jj + (uint32_t)t;
-          const int st = kQuant ? 0 : j % NS;
-          ok = wait(B_PREADY + (j & 1), (j >> 1) & 1, 213) && wait(kQuant ? B_CV : B_VFULL + st, kQuant ? (j & 1) : ((j / NS) & 1), 214);
+          const int st = kQuant ? j % NC : j % NS;
+          ok = warp_wait(bar(kQuant ? B_CV + st : B_VFULL + st), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 214);
           if (!ok) break;
-          const uint32_t v_at = sbase + (kQuant ? P::kOffCV : P::kOffV + st * P::kStage);
+          const uint32_t v_at = sbase + (kQuant ? P::kOffCV + st * P::kTile : P::kOffV + st * P::kStage);
           if constexpr (!kQuant) {  // rows behind the sequence's end hold anything, and 0 times anything may be NaN
             int32_t first, slot;
             const int keys = keys_of(w.t0 + t, first, slot);
@@ -381,35 +402,46 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               __syncwarp();
             }
           }
-          tc_fence_after();
           // 16 keys per MMA = two 8-row swizzle groups; 64 columns of d lie kKVChunk apart
           const uint64_t vd = smem_desc(v_at, P::kKVChunk, 1024, kLayoutSw128);
-          if (el) {
 #pragma unroll
-            for (int kk = 0; kk < TK / 16; ++kk)
-              mma16_ts(tmem + P::kColO, tmem + P::kColS + TK * (j & 1) + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO,
-                       kk ? 1u : (t > 0 ? 1u : 0u));
-            if (kMaySplit && split) {
+          for (int sub = 0; sub < NSUB; ++sub) {
+            if (sub >= subs || !ok) continue;
+            const uint32_t own = done[sub] + (uint32_t)t;
+            ok = warp_wait(bar(B_PREADY + 2 * sub + (own & 1)), (own >> 1) & 1, abort_flag, err, 213);
+            if (!ok) continue;
+            tc_fence_after();
+            const uint32_t p_at = tmem + P::kColS + TK * (2 * sub + (own & 1)), o_at = tmem + P::kColO + sub * DP;
+            if (el) {
 #pragma unroll
               for (int kk = 0; kk < TK / 16; ++kk)
-                mma16_ts(tmem + P::kColO, tmem + P::kColS + TK * (j & 1) + TK / 2 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4),
-                         kIdescO, 1u);
+                mma16_ts(o_at, p_at + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, kk ? 1u : (t > 0 ? 1u : 0u));
+              if (kMaySplit && split) {
+#pragma unroll
+                for (int kk = 0; kk < TK / 16; ++kk)
+                  mma16_ts(o_at, p_at + TK / 2 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, 1u);
+              }
+              tc_commit(bar(B_OREADY + 2 * sub + (own & 1)));
+              if (sub == subs - 1) tc_commit(bar(kQuant ? B_CV + NC + st : B_VEMPTY + st));
             }
-            tc_commit(bar(B_OREADY + (j & 1)));
-            tc_commit(bar(kQuant ? B_CV + 1 : B_VEMPTY + st));
+            __syncwarp();
+            // its S buffer is free once the product above is queued (the pipe runs them in order)
+            if (sub == 0) ok = k_ready(t + 2);
+            if (ok) issue_S(t + 2, sub);
           }
-          __syncwarp();
-          ok = issue_S(t + 2);  // its S buffer is free once the product above is queued (the pipe runs them in order)
         }
         jj += (uint32_t)n;
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+          if (sub < subs) done[sub] += (uint32_t)n;
       }
-    } else if (kQuant && warp >= 8) {
+    } else if (kQuant && warp >= P::kConvertFrom) {
       // =============================== the tiles of an 8-bit cache ===============================
       if constexpr (kQuant) {
         // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1)
         constexpr int UPT = DP / 16, R = P::kConvert / UPT;  // 16-byte units of a row of codes, rows of one step
-        const int tid = threadIdx.x - 256, r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
-        // the two halves of d would meet in the same banks: the second one stores its pieces the other way round
+        const int tid = threadIdx.x - P::kConvertFrom * 32, r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
+        // the two halves of d would meet in the same banks: the second one turns its pieces round
         const uint32_t to0 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + s), to1 = ch * P::kKVChunk + P::unit(r0, (u % 4) * 2 + (s ^ 1));
         uint32_t jj = 0;
         bool ok = true;
@@ -418,9 +450,9 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             const bool is_v = step > 0 && ((step & 1) == 0 || step == 2 * w.n - 1);
             const int32_t t = step == 2 * w.n - 1 ? w.n - 1 : (step + 1) / 2 - (is_v ? 1 : 0);
             const uint32_t j = jj + (uint32_t)t;
-            const int st = j % NS, done = is_v ? B_CV : B_CK;
+            const int st = j % NS, done = (is_v ? B_CV : B_CK) + j % NC;
             ok = warp_wait(bar((is_v ? B_VFULL : B_KFULL) + st), (j / NS) & 1, abort_flag, err, 412) &&
-                 warp_wait(bar(done + 1), (j & 1) ^ 1u, abort_flag, err, 413);
+                 warp_wait(bar(done + NC), ((j / NC) & 1) ^ 1u, abort_flag, err, 413);
             if (!ok) break;
             int keys = is_v ? a.tile_keys : TK;  // behind them lies what no box reaches
             if (is_v && w.t0 + t == w.tiles - 1) {  // rows behind the sequence's end hold anything
@@ -428,22 +460,26 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               keys = keys_of(w.t0 + t, first, slot);
             }
             const uint8_t* src = smem + (is_v ? P::kOffV : P::kOffK) + st * P::kStage + tid * 16;
-            uint8_t* dst = smem + (is_v ? P::kOffCV : P::kOffCK);
+            uint8_t* dst = smem + (is_v ? P::kOffCV : P::kOffCK) + j % NC * P::kTile;
 #pragma unroll
             for (int i = 0; i < TK / R; ++i) {
               uint4 c = *reinterpret_cast<const uint4*>(src + i * R * DP);
+              if (s) c = make_uint4(c.z, c.w, c.x, c.y);
               if (keys < TK && r0 + i * R >= keys) c = make_uint4(0, 0, 0, 0);
               uint4 y0, y1;
               Widen<TC>::four(c.x, y0.x, y0.y);
               Widen<TC>::four(c.y, y0.z, y0.w);
               Widen<TC>::four(c.z, y1.x, y1.y);
               Widen<TC>::four(c.w, y1.z, y1.w);
-              *reinterpret_cast<uint4*>(dst + to0 + i * R * 128) = s ? y1 : y0;
-              *reinterpret_cast<uint4*>(dst + to1 + i * R * 128) = s ? y0 : y1;
+              *reinterpret_cast<uint4*>(dst + to0 + i * R * 128) = y0;
+              *reinterpret_cast<uint4*>(dst + to1 + i * R * 128) = y1;
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(bar(done));
-            mbar_arrive(bar((is_v ? B_VEMPTY : B_KEMPTY) + st));
+            __syncwarp();
+            if (lane == 0) {  // one arrival a warp: those of 32 lanes would take as many turns at the barrier
+              mbar_arrive(bar(done));
+              mbar_arrive(bar((is_v ? B_VEMPTY : B_KEMPTY) + st));
+            }
           }
           jj += (uint32_t)w.n;
         }
@@ -460,22 +496,28 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     constexpr float kSlack = kHalfP ? 4.f : 8.f, kLift = kHalfP ? 10.f : 0.f;
     const uint64_t minus1 = pack2(-1.f, -1.f);
     constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    const uint32_t tO = tmem + lane_base + P::kColO;
-    auto group_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    uint32_t jj = 0;
+    const int sub = warp / 4, tid = threadIdx.x % 128;
+    const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16;
+    const uint32_t tO = tmem + lane_base + P::kColO + sub * DP, tS0 = tmem + lane_base + P::kColS + 2 * TK * sub;
+    const int b_sready = B_SREADY + 2 * sub, b_pready = B_PREADY + 2 * sub, b_oready = B_OREADY + 2 * sub;
+    auto group_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // of units with copies: one sub-tile
+    uint32_t jj = 0, ring = 0;  // tiles of this row tile, and of the CTA
     bool ok = true;
 
     // One piece. kCols: the columns of a tile that a thread works on, 64 over the number of copies of the unit's rows.
     auto piece = [&](auto cols_tag) -> bool {
       constexpr int kCols = decltype(cols_tag)::value, kCopies = 64 / kCols, kBlock = 128 / kCopies;
-      const int rows = w.rows(a);
-      const int row = threadIdx.x % kBlock, copy = threadIdx.x / kBlock, col0 = copy * kCols;  // the copy is the warp's
+      const int rows = w.rows(a) - sub * 128;
+      const int row = tid % kBlock, copy = tid / kBlock, col0 = copy * kCols;  // the copy is the warp's
       const bool mine = row < rows;
+      if (NSUB > 1 && rows <= 0) {  // the unit has no second tile
+        ring += (uint32_t)w.n;
+        return true;
+      }
       // ---- Q: every product with the last unit's has completed ----
       float sc = a.scale_log2e;
       if (mine) {
-        const int32_t xr = w.row0 + row, t = xr / a.group;
+        const int32_t xr = w.row0 + sub * 128 + row, t = xr / a.group;
         const T* src = reinterpret_cast<const T*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
                        ((int64_t)w.h * a.group + (xr - t * a.group)) * a.q_stride[1];
         auto eight = [&](int u0, uint4 (&q)[8]) {  // eight 16-byte units, all in flight together
@@ -526,26 +568,28 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 v[k + 1] = (x >> 16) | (y & 0xffff0000u);
               }
             }
-            *reinterpret_cast<uint4*>(smem + P::kOffQ + (u / 8) * P::kQChunk + P::unit(threadIdx.x, i)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(smem + P::kOffQ + sub * P::kQSub + (u / 8) * P::kQChunk + P::unit(tid, i)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }  // rows beyond the unit's keep what was there: no row's result depends on another's
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(bar(B_QFULL));
-      if (kCopies == 1 && warp * 32 >= rows) {  // nothing here: keep step with the barriers
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_QFULL + sub));
+      if (kCopies == 1 && warp % 4 * 32 >= rows) {  // nothing here: keep step with the barriers
+        ring += (uint32_t)w.n;
         for (int32_t t = 0; t < w.n; ++t, ++jj) {
-          if (!warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315)) return false;
-          if (lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+          if (!warp_wait(bar(b_sready + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 315)) return false;
+          if (lane == 0) mbar_arrive(bar(b_pready + (jj & 1)));
         }
         return true;
       }
-      const bool split = kMaySplit && w.tokens * a.group <= P::kRows;
+      const bool split = kMaySplit && w.tokens * a.group <= 128;
       float m_true = neg_inf(), shift = neg_inf();
       float v_ref = -80.f;  // exponent of the largest of V's scales so far
       uint64_t l2[2] = {0ull, 0ull};
-      for (int32_t t = 0; t < w.n; ++t, ++jj) {
-        const uint32_t tS = tmem + lane_base + P::kColS + TK * (jj & 1);
-        if (!warp_wait(bar(B_SREADY + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311)) return false;
+      for (int32_t t = 0; t < w.n; ++t, ++jj, ++ring) {
+        const uint32_t tS = tS0 + TK * (jj & 1);
+        if (!warp_wait(bar(b_sready + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311)) return false;
         tc_fence_after();
         uint32_t sr[kCols];
         if constexpr (kCols == 16) tmem_ld16(tS + col0, sr);
@@ -554,8 +598,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sr));
           tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
         }
-        const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + jj % P::kRing);
-        [[maybe_unused]] const float* scales = ring_scale + (jj % P::kRing) * 2 * TK + col0;
+        const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + ring % P::kRing);
+        [[maybe_unused]] const float* scales = ring_scale + (ring % P::kRing) * 2 * TK + col0;
         [[maybe_unused]] const ulonglong2 *ks = reinterpret_cast<const ulonglong2*>(scales), *vs = reinterpret_cast<const ulonglong2*>(scales + TK);
         if constexpr (kQuant) {
           const volatile uint32_t* all = reinterpret_cast<const volatile uint32_t*>(scales + TK - col0);
@@ -598,7 +642,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           l2[0] = fma2(l2[0], f2, 0ull);
           l2[1] = fma2(l2[1], f2, 0ull);
           if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
-            if (!warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312)) return false;
+            if (!warp_wait(bar(b_oready + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312)) return false;
             tc_fence_after();
             uint32_t ob[8];
 #pragma unroll 1
@@ -657,10 +701,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_PREADY + (jj & 1)));
+        if (lane == 0) mbar_arrive(bar(b_pready + (jj & 1)));
       }
       // ---- the piece's rows leave ----
-      if (!warp_wait(bar(B_OREADY + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314)) return false;
+      if (!warp_wait(bar(b_oready + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 314)) return false;
       tc_fence_after();
       float la, lb, lc, ld;
       unpack2(l2[0], la, lb);
@@ -670,7 +714,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       // a NaN score passes the maximum by and shows in the sum
       float m = (l_run != l_run && m_true < __int_as_float(0x7f800000)) ? l_run : m_true, l = l_run * rel;
       if constexpr (kCopies > 1) {
-        row_ml[threadIdx.x] = make_float2(m, l);
+        row_ml[tid] = make_float2(m, l);
         group_sync();
         float top = neg_inf();
 #pragma unroll
@@ -685,7 +729,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
         m = top;
       }
-      const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0, blockIdx.x);
+      const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0 + sub * 128, blockIdx.x);
       if (mine && copy == 0) a.ml[out + row] = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
@@ -726,9 +770,9 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           __syncwarp();
         } else {  // the copies are added up where Q was, 32 columns at a time
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + P::unit(threadIdx.x, e / 4)) = four(e);
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + P::unit(tid, e / 4)) = four(e);
           group_sync();
-          for (int x = threadIdx.x; x < rows * 8; x += 128) {
+          for (int x = tid; x < rows * 8; x += 128) {
             const int r = x / 8, u = x % 8;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -746,6 +790,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     };
     while (ok && w.next(a)) {
       const int rows = w.rows(a);
+      if constexpr (NSUB > 1) {
+        ok = piece(std::integral_constant<int, 64>());
+        continue;
+      }
       if (rows <= 32) ok = piece(std::integral_constant<int, 16>());
       else if (rows <= 64) ok = piece(std::integral_constant<int, 32>());
       else ok = piece(std::integral_constant<int, 64>());
@@ -755,7 +803,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   // ---- common exit: everyone is done with TMEM before it is released ----
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == P::kAux) {
     tc_fence_after();
     if (*abort_flag && lane == 0) {  // copies that may still be in flight land before the CTA's shared memory is reused
       const uint64_t t0 = globaltimer();

@@ -82,6 +82,8 @@ SHAPES = [  # lens, rows, Hq, Hkv, d, page, layout
     ([300, 20], [2, 6], 4, 2, 256, 16, "nhd"), ([33, 80], [3, 2], 3, 1, 3, 5, "nhd"), ([50], [4], 2, 2, 200, 10, "hnd"),
     ([40], [2], 2, 1, 1024, 4, "nhd"), ([70, 10], [2, 5], 2, 1, 37, 7, "nhd"), ([64], [2], 1, 1, 512, 16, "nhd"),
     ([45], [3], 2, 2, 32, 20, "nhd"), ([600], [40], 16, 2, 16, 8, "nhd"),
+    # more rows than a row tile holds on average, sequences with fewer among them
+    ([600, 100, 0, 300, 70], [40, 70, 33, 5, 33], 16, 2, 128, 16, "hnd"), ([1500, 64], [30, 9], 16, 1, 64, 64, "nhd"),
 ]
 
 
