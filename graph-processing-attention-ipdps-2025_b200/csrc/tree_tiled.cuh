@@ -188,15 +188,15 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(bar(B_KFULL + s), kQuant ? 33 : 1);
-      mbar_init(bar(B_KEMPTY + s), kQuant ? P::kConvert / 32 : 1);
+      mbar_init(bar(B_KEMPTY + s), kQuant ? P::kConvert / 32 : NSUB);
       mbar_init(bar(B_VFULL + s), 1);
-      mbar_init(bar(B_VEMPTY + s), kQuant ? P::kConvert / 32 : 1);
+      mbar_init(bar(B_VEMPTY + s), kQuant ? P::kConvert / 32 : NSUB);
     }
     for (int x = 0; x < NC; ++x) {
       mbar_init(bar(B_CK + x), kQuant ? P::kConvert / 32 : 1);
-      mbar_init(bar(B_CK + NC + x), 1);
+      mbar_init(bar(B_CK + NC + x), NSUB);
       mbar_init(bar(B_CV + x), kQuant ? P::kConvert / 32 : 1);
-      mbar_init(bar(B_CV + NC + x), 1);
+      mbar_init(bar(B_CV + NC + x), NSUB);
     }
     for (int x = 0; x < 2 * NSUB; ++x) {
       mbar_init(bar(B_SREADY + x), 1);
@@ -338,62 +338,69 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         }
       }
       if constexpr (kQuant) asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp == P::kAux + 1) {
-      // =============================== MMA issuer ===============================
+    } else if (warp == P::kAux + 1 || (NSUB == 2 && warp == P::kAux + 3)) {
+      // =============================== MMA issuers: one for each row tile ===============================
+      const int sub = NSUB == 2 && warp == P::kAux + 3 ? 1 : 0;
       const bool el = elect_one();
-      auto wait = [&](int b, uint32_t parity, int code) -> bool { return warp_wait(bar(b), parity, abort_flag, err, code); };
       constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
-      const uint64_t qd = smem_desc(sbase + P::kOffQ, 16, 1024, kLayoutSw128);
-      uint32_t jj = 0;
-      uint32_t done[NSUB] = {}, units[NSUB] = {};  // tiles and units of each row tile: an empty second one does not count
+      const uint64_t qd = smem_desc(sbase + P::kOffQ + sub * P::kQSub, 16, 1024, kLayoutSw128);
+      const uint32_t s_at = tmem + P::kColS + 2 * TK * sub, o_at = tmem + P::kColO + sub * DP;
+      const int b_sready = B_SREADY + 2 * sub, b_pready = B_PREADY + 2 * sub, b_oready = B_OREADY + 2 * sub;
+      uint32_t jj = 0, done = 0, unit = 0;  // tiles of the CTA, tiles and units of this row tile
       bool ok = true;
       while (ok && w.next(a)) {
         const int32_t n = w.n;
         const bool split = w.tokens * a.group <= 128;
-        const int subs = NSUB == 1 ? 1 : (w.rows(a) > 128 ? 2 : 1);
-#pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
-          if (sub < subs && ok) ok = warp_wait(bar(B_QFULL + sub), units[sub]++ & 1, abort_flag, err, 211);
-        if (!ok) break;
-        auto k_ready = [&](int32_t t) -> bool {
-          const uint32_t j = jj + (uint32_t)t;
-          return t >= n || warp_wait(bar(kQuant ? B_CK + j % NC : B_KFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 212);
+        const bool idle = NSUB == 2 && sub == 1 && w.rows(a) <= 128;  // the unit has no second tile: only the stages are handed on
+        auto k_ready = [&](uint32_t j) -> bool {
+          return warp_wait(bar(kQuant ? B_CK + j % NC : B_KFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 212);
         };
-        auto issue_S = [&](int32_t t, int sub) {
-          if (t >= n) return;
-          const uint32_t j = jj + (uint32_t)t, buf = (done[sub] + (uint32_t)t) & 1;
+        auto v_ready = [&](uint32_t j) -> bool {
+          return warp_wait(bar(kQuant ? B_CV + j % NC : B_VFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 214);
+        };
+        if (idle) {
+          for (int32_t t = 0; t < n && ok; ++t, ++jj) {
+            ok = k_ready(jj);
+            if (ok && el) mbar_arrive(bar(kQuant ? B_CK + NC + jj % NC : B_KEMPTY + jj % NS));
+            ok = ok && v_ready(jj);
+            if (ok && el) mbar_arrive(bar(kQuant ? B_CV + NC + jj % NC : B_VEMPTY + jj % NS));
+          }
+          continue;
+        }
+        ok = warp_wait(bar(B_QFULL + sub), unit & 1, abort_flag, err, 211);
+        ++unit;
+        if (!ok) break;
+        auto issue_S = [&](int32_t t) -> bool {
+          if (t >= n) return true;
+          const uint32_t j = jj + (uint32_t)t, buf = (done + (uint32_t)t) & 1;
           const int st = kQuant ? j % NC : j % NS;
+          if (!k_ready(j)) return false;
           tc_fence_after();
           const uint64_t kd = smem_desc(sbase + (kQuant ? P::kOffCK + st * P::kTile : P::kOffK + st * P::kStage), 16, 1024, kLayoutSw128);
           if (el) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {  // 16 elements (32 bytes) of the contraction per MMA
               const int c = kk / 4, in = kk % 4 * 32;
-              mma16_ss(tmem + P::kColS + TK * (2 * sub + buf), qd + (uint64_t)((sub * P::kQSub + c * P::kQChunk + in) >> 4),
-                       kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS, kk ? 1u : 0u);
+              mma16_ss(s_at + TK * buf, qd + (uint64_t)((c * P::kQChunk + in) >> 4), kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS,
+                       kk ? 1u : 0u);
             }
-            tc_commit(bar(B_SREADY + 2 * sub + buf));
-            if (sub == subs - 1) tc_commit(bar(kQuant ? B_CK + NC + st : B_KEMPTY + st));
+            tc_commit(bar(b_sready + buf));
+            tc_commit(bar(kQuant ? B_CK + NC + st : B_KEMPTY + st));
           }
           __syncwarp();
+          return true;
         };
-        for (int32_t t = 0; t < 2 && ok; ++t) {
-          ok = k_ready(t);
-          if (!ok) break;
-#pragma unroll
-          for (int sub = 0; sub < NSUB; ++sub)
-            if (sub < subs) issue_S(t, sub);
-        }
+        ok = issue_S(0) && issue_S(1);
         for (int32_t t = 0; t < n && ok; ++t) {
-          const uint32_t j = jj + (uint32_t)t;
+          const uint32_t j = jj + (uint32_t)t, own = done + (uint32_t)t;
           const int st = kQuant ? j % NC : j % NS;
-          ok = warp_wait(bar(kQuant ? B_CV + st : B_VFULL + st), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 214);
+          ok = v_ready(j);
           if (!ok) break;
           const uint32_t v_at = sbase + (kQuant ? P::kOffCV + st * P::kTile : P::kOffV + st * P::kStage);
           if constexpr (!kQuant) {  // rows behind the sequence's end hold anything, and 0 times anything may be NaN
-            int32_t first, slot;
-            const int keys = keys_of(w.t0 + t, first, slot);
-            if (keys < a.tile_keys) {
+            if (w.t0 + t == w.tiles - 1) {
+              int32_t first, slot;
+              const int keys = keys_of(w.t0 + t, first, slot);
               for (int x = keys * 8 + lane; x < TK * 8; x += 32)
 #pragma unroll
                 for (int c = 0; c < P::kChunks; ++c)
@@ -404,36 +411,27 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           }
           // 16 keys per MMA = two 8-row swizzle groups; 64 columns of d lie kKVChunk apart
           const uint64_t vd = smem_desc(v_at, P::kKVChunk, 1024, kLayoutSw128);
+          ok = warp_wait(bar(b_pready + (own & 1)), (own >> 1) & 1, abort_flag, err, 213);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t p_at = s_at + TK * (own & 1);
+          if (el) {
 #pragma unroll
-          for (int sub = 0; sub < NSUB; ++sub) {
-            if (sub >= subs || !ok) continue;
-            const uint32_t own = done[sub] + (uint32_t)t;
-            ok = warp_wait(bar(B_PREADY + 2 * sub + (own & 1)), (own >> 1) & 1, abort_flag, err, 213);
-            if (!ok) continue;
-            tc_fence_after();
-            const uint32_t p_at = tmem + P::kColS + TK * (2 * sub + (own & 1)), o_at = tmem + P::kColO + sub * DP;
-            if (el) {
+            for (int kk = 0; kk < TK / 16; ++kk)
+              mma16_ts(o_at, p_at + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, kk ? 1u : (t > 0 ? 1u : 0u));
+            if (kMaySplit && split) {
 #pragma unroll
               for (int kk = 0; kk < TK / 16; ++kk)
-                mma16_ts(o_at, p_at + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, kk ? 1u : (t > 0 ? 1u : 0u));
-              if (kMaySplit && split) {
-#pragma unroll
-                for (int kk = 0; kk < TK / 16; ++kk)
-                  mma16_ts(o_at, p_at + TK / 2 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, 1u);
-              }
-              tc_commit(bar(B_OREADY + 2 * sub + (own & 1)));
-              if (sub == subs - 1) tc_commit(bar(kQuant ? B_CV + NC + st : B_VEMPTY + st));
+                mma16_ts(o_at, p_at + TK / 2 + kk * 8, vd + (uint64_t)((kk * 16 * 128) >> 4), kIdescO, 1u);
             }
-            __syncwarp();
-            // its S buffer is free once the product above is queued (the pipe runs them in order)
-            if (sub == 0) ok = k_ready(t + 2);
-            if (ok) issue_S(t + 2, sub);
+            tc_commit(bar(b_oready + (own & 1)));
+            tc_commit(bar(kQuant ? B_CV + NC + st : B_VEMPTY + st));
           }
+          __syncwarp();
+          ok = issue_S(t + 2);  // its S buffer is free once the product above is queued (the pipe runs them in order)
         }
         jj += (uint32_t)n;
-#pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
-          if (sub < subs) done[sub] += (uint32_t)n;
+        done += (uint32_t)n;
       }
     } else if (kQuant && warp >= P::kConvertFrom) {
       // =============================== the tiles of an 8-bit cache ===============================
