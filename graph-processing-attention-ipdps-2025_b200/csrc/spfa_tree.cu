@@ -7,7 +7,6 @@ namespace spfa {
 namespace {
 
 constexpr int kCtas = 296;     // of the tensor-core context kernel: two on each of 148 SMs
-constexpr int kAnyCtas = 592;  // of the other one where d <= 64, and half as many above
 
 struct TreeLayout {
   int d_pad;
@@ -17,7 +16,7 @@ struct TreeLayout {
 TreeLayout tree_layout(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
   TreeLayout t{};
   // either context kernel must fit: which one runs is settled by the call
-  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? 128 * kCtas : tree::kAnyRows * kAnyCtas;
+  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? 128 * kCtas : 32 * 444;  // 32 rows x 3 CTAs on an SM are the most without
   t.d_pad = (c->d + 3) / 4 * 4;
   t.rows = n_rows * n_q_heads + pieces;
   t.cut = 0;
@@ -107,12 +106,12 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
     a.page_tiles = ps >= keys ? (ps + keys - 1) / keys : 0;
     a.tile_keys = ps >= keys ? keys : keys / ps * ps;
   } else {
-    a.row_tile = tree::kAnyRows;
-    a.tile_keys = tree::any_tile_keys(c->d);
+    a.row_tile = tree::any_rows(a);
+    a.tile_keys = tree::any_tile_keys(tree::any_padded(c->d));
     a.page_tiles = 0;
   }
   a.least = 1;
-  a.n_cta = grid_of(a, tiled ? kCtas / subs : c->d <= 64 ? kAnyCtas : kAnyCtas / 2);
+  a.n_cta = grid_of(a, tiled ? kCtas / subs : tree::any_ctas(c->d, a.row_tile));
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
   a.ml = reinterpret_cast<float2*>(ws + t.ml);

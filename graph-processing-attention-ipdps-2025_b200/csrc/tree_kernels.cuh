@@ -178,35 +178,55 @@ struct Walk {
 
 // ---- context kernel without tensor cores: 32-bit products, any types and any d ---------------------------------------------
 //
-// 256 threads, 16 rows, TK keys at a time in shared memory as 32-bit values. Scores: a warp takes 16 keys and a slice of d, each
-// thread 4 rows x 2 keys, so that six 16-byte shared loads feed 32 products a lane. P V: a thread owns 4 rows x 4 columns of O in
-// registers and, where d leaves threads over, a share of the keys.
-template <int DP>
+// 256 threads, 16 or 32 rows, TK keys at a time in shared memory as 32-bit values. Scores: a warp takes 16 rows x 16 keys (and, where
+// that leaves warps over, a slice of d), each thread 4 rows x 2 keys, so that six 16-byte shared loads feed 32 products a lane. P V: a
+// thread owns 4 rows x 4 columns of O in registers and, where d leaves threads over, a share of the keys. Pairs of products share an
+// instruction. A tile is a chain of short phases between barriers; other CTAs of the SM fill its gaps.
+// (float32, 16 drafted tokens of 2 x 4 heads, 4096 keys, d = 64: 37 us with 16 rows, whose K and V a unit's second row tile loads again.)
+__host__ __device__ constexpr int any_tile_keys(int dp) { return dp <= 128 ? 64 : (dp == 256 ? 32 : 16); }
+template <int DP, int R>
 struct PlanAny {
-  static constexpr int kThreads = 256, kRows = 16;
-  // A tile is a chain of short phases between barriers, and other CTAs fill the gaps: as many as shared memory takes (four where
-  // d <= 64: 16 x 8 heads over 4096 float32 keys in 25 us, with two in 37).
-  static constexpr int kCtasPerSm = DP == 64 ? 4 : DP <= 256 ? 2 : 1;
-  static constexpr int TK = DP <= 128 ? 64 : (DP == 256 ? 32 : 16);
-  static constexpr int KB = TK / 16, DS = 8 / KB;  // key blocks x slices of d = 8 warps
-  static constexpr int CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (4 * CGT);
+  static constexpr int kThreads = 256, kRows = R;
+  static constexpr int kCtasPerSm = DP == 64 ? (R == 16 ? 4 : 3) : DP <= 256 ? 2 : 1;
+  static constexpr int TK = any_tile_keys(DP);
+  static constexpr int KB = TK / 16, RB = R / 16, DS = 8 / (KB * RB);  // blocks of keys x blocks of rows x slices of d = 8 warps
+  static constexpr int RG = R / 4, CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (RG * CGT);
   static constexpr int kPitch = DP + 4;  // floats: rows start 16 bytes further round the banks
+  static constexpr int kPitchP = R + 4;
   static constexpr int kOffQ = 0, kOffK = kOffQ + kRows * kPitch * 4, kOffV = kOffK + TK * kPitch * 4;
-  static constexpr int kOffS = kOffV + TK * kPitch * 4, kOffP = kOffS + DS * kRows * TK * 4, kOffRow = kOffP + TK * 20 * 4;
+  static constexpr int kOffS = kOffV + TK * kPitch * 4, kOffP = kOffS + DS * kRows * TK * 4, kOffRow = kOffP + TK * kPitchP * 4;
   static constexpr int kOffKey = kOffRow + 3 * kRows * 4, kOffCut = kOffKey + TK * 24, kBytes = kOffCut + (int)sizeof(Cut);
+  static_assert(DS >= 1 && KS >= 1, "every warp has work");
   static_assert(KS * kRows * DP <= (TK * kPitch) * 2, "the shares of O are added up where K and V were");
 };
 
-template <int DP, class TQ, class TC>
-__global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kernel(const Call a, const int vec) {
-  using P = PlanAny<DP>;
-  constexpr int TK = P::TK, R = P::kRows, PITCH = P::kPitch;
+// Two products and sums in one instruction.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+
+template <int DP, int R, class TQ, class TC>
+__global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_kernel(const Call a, const int vec) {
+  using P = PlanAny<DP, R>;
+  constexpr int TK = P::TK, PITCH = P::kPitch, PP = P::kPitchP;
   extern __shared__ __align__(16) uint8_t smem[];
   float* Qs = reinterpret_cast<float*>(smem + P::kOffQ);
   float* Ks = reinterpret_cast<float*>(smem + P::kOffK);
   float* Vs = reinterpret_cast<float*>(smem + P::kOffV);
   float* Ss = reinterpret_cast<float*>(smem + P::kOffS);
-  float* Ps = reinterpret_cast<float*>(smem + P::kOffP);  // [key][20]
+  float* Ps = reinterpret_cast<float*>(smem + P::kOffP);  // [key][PP]
   float* row_m = reinterpret_cast<float*>(smem + P::kOffRow);
   float* row_l = row_m + R;
   float* row_f = row_l + R;
@@ -242,14 +262,12 @@ __global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kern
       row_m[tid] = neg_inf();
       row_l[tid] = 0.f;
     }
-    float o[4][P::NCG][4];
+    uint64_t o[4][P::NCG][2];  // pairs of columns
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int g = 0; g < P::NCG; ++g)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[r][g][i] = 0.f;
-    const int rg = tid & 3, cg = (tid >> 2) % P::CGT, ks = tid / (4 * P::CGT);
+      for (int g = 0; g < P::NCG; ++g) o[r][g][0] = o[r][g][1] = 0ull;
+    const int rg = tid % P::RG, cg = (tid / P::RG) % P::CGT, ks = tid / (P::RG * P::CGT);
 
     auto page_at = [&](int32_t t) -> int32_t {  // of this thread's key of tile t: looked up a tile ahead
       const int64_t p = (int64_t)t * TK + tid;
@@ -309,32 +327,33 @@ __global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kern
       }
       __syncthreads();
       {  // scores
-        const int kb = warp % P::KB, ds = warp / P::KB, r4 = lane >> 3, kg = lane & 7;
-        const float* qp = Qs + r4 * 4 * PITCH + ds * (DP / P::DS);
+        const int kb = warp % P::KB, rb = warp / P::KB % P::RB, ds = warp / (P::KB * P::RB), r0 = rb * 16 + (lane >> 3) * 4, kg = lane & 7;
+        const float* qp = Qs + r0 * PITCH + ds * (DP / P::DS);
         const float* kp = Ks + (kb * 16 + kg) * PITCH + ds * (DP / P::DS);
-        float s[4][2] = {};
+        uint64_t s[4][2] = {};
 #pragma unroll 4
         for (int e = 0; e < DP / P::DS; e += 4) {
-          const float4 k0 = *reinterpret_cast<const float4*>(kp + e);
-          const float4 k1 = *reinterpret_cast<const float4*>(kp + 8 * PITCH + e);
+          const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(kp + e);
+          const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(kp + 8 * PITCH + e);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float4 q = *reinterpret_cast<const float4*>(qp + r * PITCH + e);
-            s[r][0] = fmaf(q.x, k0.x, fmaf(q.y, k0.y, fmaf(q.z, k0.z, fmaf(q.w, k0.w, s[r][0]))));
-            s[r][1] = fmaf(q.x, k1.x, fmaf(q.y, k1.y, fmaf(q.z, k1.z, fmaf(q.w, k1.w, s[r][1]))));
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(qp + r * PITCH + e);
+            s[r][0] = pair_fma(q.y, k0.y, pair_fma(q.x, k0.x, s[r][0]));
+            s[r][1] = pair_fma(q.y, k1.y, pair_fma(q.x, k1.x, s[r][1]));
           }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          Ss[(ds * R + r4 * 4 + r) * TK + kb * 16 + kg] = s[r][0];
-          Ss[(ds * R + r4 * 4 + r) * TK + kb * 16 + kg + 8] = s[r][1];
+          const float2 x = halves(s[r][0]), y = halves(s[r][1]);
+          Ss[(ds * R + r0 + r) * TK + kb * 16 + kg] = x.x + x.y;
+          Ss[(ds * R + r0 + r) * TK + kb * 16 + kg + 8] = y.x + y.y;
         }
       }
       __syncthreads();
 #pragma unroll
-      for (int rr = 0; rr < 2; ++rr) {  // softmax: a warp takes two rows
+      for (int rr = 0; rr < R / 8; ++rr) {  // softmax: a warp takes two rows or four
         constexpr int KL = (TK + 31) / 32;
-        const int r = warp * 2 + rr;
+        const int r = warp * (R / 8) + rr;
         float s[KL], top = neg_inf();
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
@@ -358,7 +377,7 @@ __global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kern
           const int key = lane + 32 * i;
           const float p = fast_exp2(s[i] - ref);
           sum += p;
-          if (key < TK) Ps[key * 20 + r] = p;
+          if (key < TK) Ps[key * PP + r] = p;
         }
 #pragma unroll
         for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o2);
@@ -375,23 +394,25 @@ __global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kern
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float f = row_f[rg * 4 + r];
+          const uint64_t f2 = pair(f, f);
 #pragma unroll
           for (int g = 0; g < P::NCG; ++g)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[r][g][i] *= f;
+            for (int i = 0; i < 2; ++i) o[r][g][i] = pair_fma(o[r][g][i], f2, 0ull);
         }
         constexpr int KPS = TK / P::KS;
 #pragma unroll 4
         for (int key = ks * KPS; key < ks * KPS + KPS; ++key) {
-          const float4 p = *reinterpret_cast<const float4*>(Ps + key * 20 + rg * 4);
+          const float4 p = *reinterpret_cast<const float4*>(Ps + key * PP + rg * 4);
+          const uint64_t p2[4] = {pair(p.x, p.x), pair(p.y, p.y), pair(p.z, p.z), pair(p.w, p.w)};
 #pragma unroll
           for (int g = 0; g < P::NCG; ++g) {
-            const float4 v = *reinterpret_cast<const float4*>(Vs + key * PITCH + (g * P::CGT + cg) * 4);
-            const float pr[4] = {p.x, p.y, p.z, p.w}, vv[4] = {v.x, v.y, v.z, v.w};
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Vs + key * PITCH + (g * P::CGT + cg) * 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[r][g][i] = fmaf(pr[r], vv[i], o[r][g][i]);
+            for (int r = 0; r < 4; ++r) {
+              o[r][g][0] = pair_fma(p2[r], v.x, o[r][g][0]);
+              o[r][g][1] = pair_fma(p2[r], v.y, o[r][g][1]);
+            }
           }
         }
       }
@@ -403,8 +424,7 @@ __global__ void __launch_bounds__(256, PlanAny<DP>::kCtasPerSm) context_any_kern
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int g = 0; g < P::NCG; ++g)
-        *reinterpret_cast<float4*>(Os + (ks * R + rg * 4 + r) * DP + (g * P::CGT + cg) * 4) =
-            make_float4(o[r][g][0], o[r][g][1], o[r][g][2], o[r][g][3]);
+        *reinterpret_cast<ulonglong2*>(Os + (ks * R + rg * 4 + r) * DP + (g * P::CGT + cg) * 4) = make_ulonglong2(o[r][g][0], o[r][g][1]);
     __syncthreads();
     const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0, blockIdx.x);
     for (int x = tid; x < rows * (DP / 4); x += 256) {
@@ -599,18 +619,28 @@ __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArg
       L = L * f + sum;
 #pragma unroll
       for (int e = 0; e < NC * VE; ++e) acc[e] *= f;
-#pragma unroll 4
-      for (int k = 0; k < np; ++k) {
-        const float wk = __shfl_sync(kFullMask, wgt, k);
-        const float* src = a.O + (row + (int64_t)k * a.row_tile) * a.d_pad;
+      constexpr int PB = NC * VE <= 8 ? 8 : 2;  // pieces whose rows are in flight together
+      for (int k0 = 0; k0 < np; k0 += PB) {
+        float y[PB][NC * VE];
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-          if (col(i) < d) {
-            float y[VE];
-            load_vec<float, VE>(src + col(i), y);
+        for (int k = 0; k < PB; ++k) {
+          const float* src = a.O + (row + (int64_t)(k0 + k) * a.row_tile) * a.d_pad;
 #pragma unroll
-            for (int e = 0; e < VE; ++e) acc[i * VE + e] = fmaf(wk, y[e], acc[i * VE + e]);
+          for (int i = 0; i < NC; ++i) {
+            float z[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) z[e] = 0.f;
+            if (k0 + k < np && col(i) < d) load_vec<float, VE>(src + col(i), z);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) y[k][i * VE + e] = z[e];
           }
+        }
+#pragma unroll
+        for (int k = 0; k < PB; ++k) {
+          const float wk = __shfl_sync(kFullMask, wgt, (k0 + k) & 31);
+#pragma unroll
+          for (int e = 0; e < NC * VE; ++e) acc[e] = fmaf(k0 + k < np ? wk : 0.f, y[k][e], acc[e]);
+        }
       }
       M = top;
     }

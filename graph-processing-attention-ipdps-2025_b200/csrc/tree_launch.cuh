@@ -19,8 +19,11 @@ bool usable_bf16(const spfa_kv_cache* c, int subs);
 
 constexpr int kTiledKeys = 64;  // a tile of context_tiled_kernel
 
-constexpr int kAnyRows = 16;  // row tile of context_any_kernel
-inline int any_tile_keys(int d) { return d <= 128 ? 64 : (d <= 256 ? 32 : 16); }
+// Units and grid of context_any_kernel for rows of d elements: 32 rows where a sequence has more than 16 on average and a CTA's shared
+// memory holds them.
+inline int any_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : d <= 512 ? 512 : 1024; }
+inline int any_rows(const Call& a) { return a.c.d <= 128 && a.n_rows * a.group > 16LL * a.c.n_seq ? 32 : 16; }
+inline int any_ctas(int d, int rows) { return 148 * (d <= 64 ? (rows == 16 ? 4 : 3) : d <= 256 ? 2 : 1); }
 
 // Opts a kernel into its dynamic shared memory, once per device and kernel.
 template <auto kernel>
@@ -34,11 +37,11 @@ bool opt_in(int bytes) {
   return true;
 }
 
-template <int DP, class TQ, class TC>
+template <int DP, int R, class TQ, class TC>
 int launch_context_any(const Call& a, bool vec, cudaStream_t st) {
-  using P = PlanAny<DP>;
-  if (!opt_in<context_any_kernel<DP, TQ, TC>>(P::kBytes)) return SPFA_ERR_LAUNCH;
-  context_any_kernel<DP, TQ, TC><<<(unsigned)a.n_cta, P::kThreads, P::kBytes, st>>>(a, vec ? 1 : 0);
+  using P = PlanAny<DP, R>;
+  if (!opt_in<context_any_kernel<DP, R, TQ, TC>>(P::kBytes)) return SPFA_ERR_LAUNCH;
+  context_any_kernel<DP, R, TQ, TC><<<(unsigned)a.n_cta, P::kThreads, P::kBytes, st>>>(a, vec ? 1 : 0);
   g_launches.fetch_add(1);
   return launch_status();
 }
@@ -96,11 +99,12 @@ int launch_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
   const int d = a.c.d;
   if (a.direct) return launch_direct<TQ, TC>(a, g, st);
   int rc = SPFA_OK;
-  if (d <= 64) rc = launch_context_any<64, TQ, TC>(a, vec, st);
-  else if (d <= 128) rc = launch_context_any<128, TQ, TC>(a, vec, st);
-  else if (d <= 256) rc = launch_context_any<256, TQ, TC>(a, vec, st);
-  else if (d <= 512) rc = launch_context_any<512, TQ, TC>(a, vec, st);
-  else rc = launch_context_any<1024, TQ, TC>(a, vec, st);
+  const bool wide = a.row_tile == 32;
+  if (d <= 64) rc = wide ? launch_context_any<64, 32, TQ, TC>(a, vec, st) : launch_context_any<64, 16, TQ, TC>(a, vec, st);
+  else if (d <= 128) rc = wide ? launch_context_any<128, 32, TQ, TC>(a, vec, st) : launch_context_any<128, 16, TQ, TC>(a, vec, st);
+  else if (d <= 256) rc = launch_context_any<256, 16, TQ, TC>(a, vec, st);
+  else if (d <= 512) rc = launch_context_any<512, 16, TQ, TC>(a, vec, st);
+  else rc = launch_context_any<1024, 16, TQ, TC>(a, vec, st);
   return rc != SPFA_OK ? rc : launch_merge_any<TQ, TC>(a, g, vec, st);
 }
 
