@@ -16,7 +16,7 @@ struct TreeLayout {
 TreeLayout tree_layout(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_heads) {
   TreeLayout t{};
   // either context kernel must fit: which one runs is settled by the call
-  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? 128 * kCtas : 32 * 444;  // 32 rows x 3 CTAs on an SM are the most without
+  const int64_t pieces = (dtype != SPFA_DTYPE_F32 && c->d <= 128) ? 128 * kCtas : 32 * kCtas;
   t.d_pad = (c->d + 3) / 4 * 4;
   t.rows = n_rows * n_q_heads + pieces;
   t.cut = 0;
@@ -111,7 +111,7 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
     a.page_tiles = 0;
   }
   a.least = 1;
-  a.n_cta = grid_of(a, tiled ? kCtas / subs : tree::any_ctas(c->d, a.row_tile));
+  a.n_cta = grid_of(a, tiled ? kCtas / subs : tree::any_ctas(c->d));
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);
   a.ml = reinterpret_cast<float2*>(ws + t.ml);

@@ -178,19 +178,21 @@ struct Walk {
 
 // ---- context kernel without tensor cores: 32-bit products, any types and any d ---------------------------------------------
 //
-// 256 threads, 16 or 32 rows, TK keys at a time in shared memory as 32-bit values. Scores: a warp takes 16 rows x 16 keys (and, where
-// that leaves warps over, a slice of d), each thread 4 rows x 2 keys, so that six 16-byte shared loads feed 32 products a lane. P V: a
-// thread owns 4 rows x 4 columns of O in registers and, where d leaves threads over, a share of the keys. Pairs of products share an
-// instruction. A tile is a chain of short phases between barriers; other CTAs of the SM fill its gaps.
+// 256 threads, 16 or 32 rows, TK keys at a time in shared memory as 32-bit values. Shared memory feeds the products, so a thread takes
+// many rows: for the scores 8 rows x 2 keys of a slice of d (d <= 128; a warp reads 64 keys, and Q by broadcast), for P V 8 rows x 4
+// columns of O in registers and a share of the keys. Larger d leaves room for fewer keys: 4 rows x 2 keys, 4 rows x 4 columns. Pairs of
+// products share an instruction. A tile is a chain of short phases between barriers; other CTAs of the SM fill its gaps.
 // (float32, 16 drafted tokens of 2 x 4 heads, 4096 keys, d = 64: 37 us with 16 rows, whose K and V a unit's second row tile loads again.)
 __host__ __device__ constexpr int any_tile_keys(int dp) { return dp <= 128 ? 64 : (dp == 256 ? 32 : 16); }
 template <int DP, int R>
 struct PlanAny {
   static constexpr int kThreads = 256, kRows = R;
-  static constexpr int kCtasPerSm = DP == 64 ? (R == 16 ? 4 : 3) : DP <= 256 ? 2 : 1;
+  static constexpr int kCtasPerSm = DP <= 256 ? 2 : 1;
   static constexpr int TK = any_tile_keys(DP);
-  static constexpr int KB = TK / 16, RB = R / 16, DS = 8 / (KB * RB);  // blocks of keys x blocks of rows x slices of d = 8 warps
-  static constexpr int RG = R / 4, CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (RG * CGT);
+  // scores: KB blocks of keys x RB blocks of rows x DS slices of d = 8 warps; TR rows of a thread, here and in P V
+  static constexpr bool kTall = TK == 64;
+  static constexpr int TR = kTall ? 8 : 4, KB = kTall ? 1 : TK / 16, RB = kTall ? R / 8 : R / 16, DS = 8 / (KB * RB);
+  static constexpr int RG = R / TR, CGT = DP / 4 < 64 ? DP / 4 : 64, NCG = DP / 4 / CGT, KS = 256 / (RG * CGT);
   static constexpr int kPitch = DP + 4;  // floats: rows start 16 bytes further round the banks
   static constexpr int kPitchP = R + 4;
   static constexpr int kOffQ = 0, kOffK = kOffQ + kRows * kPitch * 4, kOffV = kOffK + TK * kPitch * 4;
@@ -262,12 +264,13 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
       row_m[tid] = neg_inf();
       row_l[tid] = 0.f;
     }
-    uint64_t o[4][P::NCG][2];  // pairs of columns
+    constexpr int TR = P::TR;
+    uint64_t o[TR][P::NCG][2];  // pairs of columns
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < TR; ++r)
 #pragma unroll
       for (int g = 0; g < P::NCG; ++g) o[r][g][0] = o[r][g][1] = 0ull;
-    const int rg = tid % P::RG, cg = (tid / P::RG) % P::CGT, ks = tid / (P::RG * P::CGT);
+    const int cg = tid % P::CGT, rg = tid / P::CGT % P::RG, ks = tid / (P::RG * P::CGT);
 
     auto page_at = [&](int32_t t) -> int32_t {  // of this thread's key of tile t: looked up a tile ahead
       const int64_t p = (int64_t)t * TK + tid;
@@ -326,7 +329,29 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
         *reinterpret_cast<float4*>(Vs + key * PITCH + e) = make_float4(v[0], v[1], v[2], v[3]);
       }
       __syncthreads();
-      {  // scores
+      if constexpr (P::kTall) {  // scores
+        const int rb = warp % P::RB, ds = warp / P::RB;
+        const float* qp = Qs + rb * 8 * PITCH + ds * (DP / P::DS);
+        const float* kp = Ks + lane * PITCH + ds * (DP / P::DS);
+        uint64_t s[8][2] = {};
+#pragma unroll 2
+        for (int e = 0; e < DP / P::DS; e += 4) {
+          const ulonglong2 k0 = *reinterpret_cast<const ulonglong2*>(kp + e);
+          const ulonglong2 k1 = *reinterpret_cast<const ulonglong2*>(kp + 32 * PITCH + e);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(qp + r * PITCH + e);
+            s[r][0] = pair_fma(q.y, k0.y, pair_fma(q.x, k0.x, s[r][0]));
+            s[r][1] = pair_fma(q.y, k1.y, pair_fma(q.x, k1.x, s[r][1]));
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float2 x = halves(s[r][0]), y = halves(s[r][1]);
+          Ss[(ds * R + rb * 8 + r) * TK + lane] = x.x + x.y;
+          Ss[(ds * R + rb * 8 + r) * TK + lane + 32] = y.x + y.y;
+        }
+      } else {
         const int kb = warp % P::KB, rb = warp / P::KB % P::RB, ds = warp / (P::KB * P::RB), r0 = rb * 16 + (lane >> 3) * 4, kg = lane & 7;
         const float* qp = Qs + r0 * PITCH + ds * (DP / P::DS);
         const float* kp = Ks + (kb * 16 + kg) * PITCH + ds * (DP / P::DS);
@@ -350,50 +375,62 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
         }
       }
       __syncthreads();
+      {  // softmax: a warp takes two rows or four, side by side
+        constexpr int KL = (TK + 31) / 32, N = R / 8;
+        float x[N][KL], top[N], m_old[N], sum[N];
 #pragma unroll
-      for (int rr = 0; rr < R / 8; ++rr) {  // softmax: a warp takes two rows or four
-        constexpr int KL = (TK + 31) / 32;
-        const int r = warp * (R / 8) + rr;
-        float s[KL], top = neg_inf();
+        for (int rr = 0; rr < N; ++rr) {
+          const int r = warp * N + rr;
+          top[rr] = m_old[rr] = row_m[r];
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          const int key = lane + 32 * i;
-          s[i] = neg_inf();
-          if (key < TK && k_at[key] >= 0) {
-            float x = 0.f;
+          for (int i = 0; i < KL; ++i) {
+            const int key = lane + 32 * i;
+            x[rr][i] = neg_inf();
+            if (key < TK && k_at[key] >= 0) {
+              float y = 0.f;
 #pragma unroll
-            for (int ds = 0; ds < P::DS; ++ds) x += Ss[(ds * R + r) * TK + key];
-            s[i] = x * a.scale_log2e;
+              for (int ds = 0; ds < P::DS; ++ds) y += Ss[(ds * R + r) * TK + key];
+              x[rr][i] = y * a.scale_log2e;
+            }
+            top[rr] = max_nan(top[rr], x[rr][i]);
           }
-          top = max_nan(top, s[i]);
         }
 #pragma unroll
-        for (int o2 = 16; o2 > 0; o2 >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o2));
-        const float m_old = row_m[r], m_new = max_nan(m_old, top);
-        const float ref = m_new == neg_inf() ? 0.f : m_new;  // nothing seen yet: every exponent stays -inf
-        float sum = 0.f;
+        for (int o2 = 16; o2 > 0; o2 >>= 1)
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
-          const int key = lane + 32 * i;
-          const float p = fast_exp2(s[i] - ref);
-          sum += p;
-          if (key < TK) Ps[key * PP + r] = p;
+          for (int rr = 0; rr < N; ++rr) top[rr] = max_nan(top[rr], __shfl_xor_sync(kFullMask, top[rr], o2));
+#pragma unroll
+        for (int rr = 0; rr < N; ++rr) {
+          const float ref = top[rr] == neg_inf() ? 0.f : top[rr];  // nothing seen yet: every exponent stays -inf
+          sum[rr] = 0.f;
+#pragma unroll
+          for (int i = 0; i < KL; ++i) {
+            const int key = lane + 32 * i;
+            const float p = fast_exp2(x[rr][i] - ref);
+            sum[rr] += p;
+            if (key < TK) Ps[key * PP + warp * N + rr] = p;
+          }
         }
 #pragma unroll
-        for (int o2 = 16; o2 > 0; o2 >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o2);
-        __syncwarp();
+        for (int o2 = 16; o2 > 0; o2 >>= 1)
+#pragma unroll
+          for (int rr = 0; rr < N; ++rr) sum[rr] += __shfl_xor_sync(kFullMask, sum[rr], o2);
         if (lane == 0) {
-          const float f = fast_exp2(m_old - ref);
-          row_f[r] = f;
-          row_l[r] = row_l[r] * f + sum;
-          row_m[r] = m_new;
+#pragma unroll
+          for (int rr = 0; rr < N; ++rr) {
+            const int r = warp * N + rr;
+            const float f = fast_exp2(m_old[rr] - (top[rr] == neg_inf() ? 0.f : top[rr]));
+            row_f[r] = f;
+            row_l[r] = row_l[r] * f + sum[rr];
+            row_m[r] = top[rr];
+          }
         }
       }
       __syncthreads();
       {  // O = O f + P V
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = row_f[rg * 4 + r];
+        for (int r = 0; r < TR; ++r) {
+          const float f = row_f[rg * TR + r];
           const uint64_t f2 = pair(f, f);
 #pragma unroll
           for (int g = 0; g < P::NCG; ++g)
@@ -401,15 +438,22 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
             for (int i = 0; i < 2; ++i) o[r][g][i] = pair_fma(o[r][g][i], f2, 0ull);
         }
         constexpr int KPS = TK / P::KS;
-#pragma unroll 4
+#pragma unroll 2
         for (int key = ks * KPS; key < ks * KPS + KPS; ++key) {
-          const float4 p = *reinterpret_cast<const float4*>(Ps + key * PP + rg * 4);
-          const uint64_t p2[4] = {pair(p.x, p.x), pair(p.y, p.y), pair(p.z, p.z), pair(p.w, p.w)};
+          uint64_t p2[TR];
+#pragma unroll
+          for (int r = 0; r < TR; r += 4) {
+            const float4 p = *reinterpret_cast<const float4*>(Ps + key * PP + rg * TR + r);
+            p2[r] = pair(p.x, p.x);
+            p2[r + 1] = pair(p.y, p.y);
+            p2[r + 2] = pair(p.z, p.z);
+            p2[r + 3] = pair(p.w, p.w);
+          }
 #pragma unroll
           for (int g = 0; g < P::NCG; ++g) {
             const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(Vs + key * PITCH + (g * P::CGT + cg) * 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < TR; ++r) {
               o[r][g][0] = pair_fma(p2[r], v.x, o[r][g][0]);
               o[r][g][1] = pair_fma(p2[r], v.y, o[r][g][1]);
             }
@@ -421,10 +465,10 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
     __syncthreads();
     float* Os = Ks;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < TR; ++r)
 #pragma unroll
       for (int g = 0; g < P::NCG; ++g)
-        *reinterpret_cast<ulonglong2*>(Os + (ks * R + rg * 4 + r) * DP + (g * P::CGT + cg) * 4) = make_ulonglong2(o[r][g][0], o[r][g][1]);
+        *reinterpret_cast<ulonglong2*>(Os + (ks * R + rg * TR + r) * DP + (g * P::CGT + cg) * 4) = make_ulonglong2(o[r][g][0], o[r][g][1]);
     __syncthreads();
     const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0, blockIdx.x);
     for (int x = tid; x < rows * (DP / 4); x += 256) {

@@ -23,7 +23,7 @@ constexpr int kTiledKeys = 64;  // a tile of context_tiled_kernel
 // memory holds them.
 inline int any_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : d <= 512 ? 512 : 1024; }
 inline int any_rows(const Call& a) { return a.c.d <= 128 && a.n_rows * a.group > 16LL * a.c.n_seq ? 32 : 16; }
-inline int any_ctas(int d, int rows) { return 148 * (d <= 64 ? (rows == 16 ? 4 : 3) : d <= 256 ? 2 : 1); }
+inline int any_ctas(int d) { return 148 * (d <= 256 ? 2 : 1); }
 
 // Opts a kernel into its dynamic shared memory, once per device and kernel.
 template <auto kernel>
