@@ -42,9 +42,11 @@ bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t*
   return dtype == SPFA_DTYPE_F16 ? tree::usable_f16(c, subs) : tree::usable_bf16(c, subs);
 }
 
-// Calls that direct_kernel takes: its CTAs, one on an SM, walk their keys in few rounds. The page lists bound the keys; lens is not
-// known here.
-constexpr double kDirectRounds = 2;
+// Calls that direct_kernel takes: its CTAs, one on an SM, have their keys in flight at once. The page lists bound the keys; lens is
+// not known here. One round against the two kernels (32 query heads of 128, 8 key heads; us): a token over 200 bfloat16 keys
+// 11.0 : 12.1, over 500 e4m3 keys 13.1 : 13.2, 16 tokens over 200 bfloat16 keys each 11.6 : 19.4. Two rounds: 500 bfloat16 keys
+// 19.0 : 12.1, 16 such tokens 19.7 : 21.2, 200 float32 keys 18.3 : 12.4.
+constexpr double kDirectRounds = 1;
 bool direct_call(const tree::Call& a, const spfa_kv_cache* c, bool vec) {
   const int size = dtype_bytes(c->dtype);
   if (!vec || c->d > 128 || !cache_rows_align(c, 16 / size)) return false;
@@ -55,8 +57,8 @@ bool direct_call(const tree::Call& a, const spfa_kv_cache* c, bool vec) {
 
 // One wave of CTAs, or as many as there can be shares of the list: lens is not known here, the page lists bound it.
 int grid_of(const tree::Call& a, int ctas) {
-  const double tiles = (double)a.tiles_of(a.c.capacity), rows = (double)a.n_rows * a.group / a.row_tile + a.c.n_seq;
-  const double most = tiles * rows * a.c.n_heads / a.least;
+  const double tiles = (double)a.tiles_of(a.c.capacity), rows = (double)a.n_rows * a.group / a.unit_rows + a.c.n_seq;
+  const double most = tiles * rows * a.c.n_heads;
   return most < ctas ? (most < 1 ? 1 : (int)most) : ctas;
 }
 
@@ -110,7 +112,8 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
     a.tile_keys = tree::any_tile_keys(tree::any_padded(c->d));
     a.page_tiles = 0;
   }
-  a.least = 1;
+  // whole tokens, so that a warp of the merge can take rows of one unit, where that leaves less than an eighth of the tile unused
+  a.unit_rows = a.group * 8 <= a.row_tile ? a.row_tile / a.group * a.group : a.row_tile;
   a.n_cta = grid_of(a, tiled ? kCtas / subs : tree::any_ctas(c->d));
   char* ws = static_cast<char*>(workspace);
   a.cut = reinterpret_cast<int64_t*>(ws + t.cut);

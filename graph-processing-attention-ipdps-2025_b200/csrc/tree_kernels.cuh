@@ -33,9 +33,9 @@ struct Call {
   int32_t n_q_heads, group;  // group = query heads of a key head
   float scale_log2e;
   // cutting the list of key tiles
-  int32_t row_tile, tile_keys;  // rows of a unit, keys of a tile
+  int32_t row_tile, tile_keys;  // rows that a CTA has room for, keys of a tile
+  int32_t unit_rows;            // rows of a unit: whole tokens where row_tile holds one
   int32_t page_tiles;           // tiles of a page (pages of tile_keys positions and more), 0: a tile spans whole pages
-  int32_t least;                // key tiles that a CTA takes at least
   int32_t n_cta;                // grid of the context kernel
   int32_t direct;               // the call runs as one launch of direct_kernel
   // workspace
@@ -49,7 +49,7 @@ struct Call {
     const int64_t full = len / c.page_size, rest = len - full * c.page_size;
     return full * page_tiles + (rest + tile_keys - 1) / tile_keys;
   }
-  __device__ __forceinline__ int64_t row_tiles(int64_t tokens) const { return (tokens * group + row_tile - 1) / row_tile; }
+  __device__ __forceinline__ int64_t row_tiles(int64_t tokens) const { return (tokens * group + unit_rows - 1) / unit_rows; }
   // Key tiles of all units of sequence b.
   __device__ __forceinline__ int64_t weight(int32_t b) const {
     int64_t begin, end;
@@ -91,7 +91,6 @@ __device__ __forceinline__ void block_cut(const Call& a, Cut* s) {
 #pragma unroll
   for (int w = 0; w < NT / 32; ++w) total += s->warp_sum[w];
   int64_t chunk = (total + a.n_cta - 1) / a.n_cta;
-  if (chunk < a.least) chunk = a.least;
   const int64_t first = (int64_t)blockIdx.x * chunk;
   if (threadIdx.x == 0) {
     s->first = first < total ? first : total;
@@ -167,12 +166,12 @@ struct Walk {
     n = tiles - t0 < last - at ? tiles - t0 : (int32_t)(last - at);
     const uint32_t rt = (uint32_t)a.row_tiles(tokens);
     h = (int32_t)(u / rt);
-    row0 = (int32_t)(u - (uint32_t)h * rt) * a.row_tile;
+    row0 = (int32_t)(u - (uint32_t)h * rt) * a.unit_rows;
     return true;
   }
   __device__ __forceinline__ int rows(const Call& a) const {  // of the unit
     const int32_t left = tokens * a.group - row0;
-    return left < a.row_tile ? left : a.row_tile;
+    return left < a.unit_rows ? left : a.unit_rows;
   }
 };
 
@@ -488,8 +487,10 @@ __global__ void __launch_bounds__(256, PlanAny<DP, R>::kCtasPerSm) context_any_k
 
 // ---- merge kernel -----------------------------------------------------------------------------------------------------------
 //
-// One warp per row; a lane holds columns (i * 32 + lane) * VE. The drafted keys come first: they need nothing of the context
-// kernel, so their loads run while it drains. Four keys at a time keep eight row loads in flight.
+// One warp per token and GR query heads of a key head (the rows); a lane holds columns (i * 32 + lane) * VE. The drafted keys come
+// first: they need nothing of the context kernel, so their loads run while it drains. A warp is a chain of dependent loads, so many
+// are in flight together: four keys of K and of V, and the pieces' O rows eight at a time. Four rows share the loads of K and V and the
+// lookups; calls that leave the machine empty take one row a warp instead (kMergeRows).
 struct MergeArgs {
   const uint8_t* mask;
   int64_t mask_width;
@@ -541,58 +542,71 @@ __device__ __forceinline__ void finish_row(const Call& a, const MergeArgs& g, in
   }
 }
 
-template <class TQ, class TC, int VE, int NC>
+template <class TQ, class TC, int VE, int NC, int GR>
 __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArgs g) {
+  constexpr int NE = NC * VE;
   const int lane = threadIdx.x & 31;
-  const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t n = warp / a.n_q_heads;
-  const int32_t hq = (int32_t)(warp - n * a.n_q_heads);
+  const uint32_t warp = blockIdx.x * 4 + (threadIdx.x >> 5), parts = (uint32_t)(a.group + GR - 1) / GR, per_row = parts * (uint32_t)a.c.n_heads;
+  const int64_t n = warp / per_row;
+  const int32_t in = (int32_t)(warp - (uint32_t)n * per_row), h = in / (int32_t)parts, g0 = (in - h * (int32_t)parts) * GR;
+  const int rows = GR == 1 ? 1 : min(GR, a.group - g0);
+  const int32_t hq = h * a.group + g0;
   const int32_t b = n < a.n_rows ? sequence_of(a.cu_rows, a.c.n_seq, n) : -1;
   if (b < 0) return;
   int64_t begin, end;
   rows_of(a.cu_rows, b, a.n_rows, begin, end);
   const int64_t tokens = end - begin, len = a.c.len_of(b);
-  const int32_t h = hq / a.group;
   const int d = a.c.d;
 
-  float q[NC * VE], acc[NC * VE];
-  float M = neg_inf(), L = 0.f;
+  float q[GR][NE], acc[GR][NE], M[GR], L[GR];
   auto col = [&](int i) { return (i * 32 + lane) * VE; };
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    float x[VE];
+  for (int r = 0; r < GR; ++r) {
+    M[r] = neg_inf();
+    L[r] = 0.f;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) x[e] = acc[i * VE + e] = 0.f;
-    if (col(i) < d) load_vec<TQ, VE>(reinterpret_cast<const TQ*>(a.Q) + n * a.q_stride[0] + hq * a.q_stride[1] + col(i), x);
+    for (int i = 0; i < NC; ++i) {
+      float x[VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) q[i * VE + e] = x[e];
+      for (int e = 0; e < VE; ++e) x[e] = acc[r][i * VE + e] = 0.f;
+      if (r < rows && col(i) < d)
+        load_vec<TQ, VE>(reinterpret_cast<const TQ*>(a.Q) + n * a.q_stride[0] + (hq + r) * a.q_stride[1] + col(i), x);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) q[r][i * VE + e] = x[e];
+    }
   }
 
-  constexpr int KB = NC * VE <= 8 ? 4 : 1;  // keys at a time: as registers allow
+  constexpr int KB = NE <= 8 ? 4 : 1;  // keys at a time: as registers allow
   const int64_t cols = tokens < g.mask_width ? tokens : g.mask_width;
   for (int64_t j0 = 0; j0 < cols; j0 += 32) {
     const bool on = j0 + lane < cols && __ldg(g.mask + n * g.mask_width + j0 + lane) != 0;
     // each lane finds the page of its own key, before the keys are taken one after the other
     const int64_t p = len + j0 + lane;
     const int32_t my_page = on ? a.c.page_of(b, p) : -1;
-    const int32_t my_slot = on ? a.c.slot_of(p) : 0;
+    const int32_t my_slot = my_page >= 0 ? a.c.slot_of(p) : 0;
+    const int64_t my_k = my_page >= 0 ? a.c.K.at(my_page, my_slot, h) : 0, my_v = my_page >= 0 ? a.c.V.at(my_page, my_slot, h) : 0;
+    float my_fk = 1.f, my_fv = 1.f;
+    if constexpr (IsByte<TC>::value) {
+      if (my_page >= 0) {
+        my_fk = a.c.K.scale[a.c.K.scale_at(my_page, my_slot, h)];
+        my_fv = a.c.V.scale[a.c.V.scale_at(my_page, my_slot, h)];
+      }
+    }
     unsigned bits = __ballot_sync(kFullMask, my_page >= 0);
     while (bits) {
-      float k[KB][NC * VE], v[KB][NC * VE], s[KB], fv[KB];
+      float k[KB][NE], v[KB][NE], s[KB][GR], fk[KB], fv[KB];
       int taken = 0;
 #pragma unroll
       for (int x = 0; x < KB; ++x) {
-        s[x] = 0.f;
-        fv[x] = 1.f;
+        fk[x] = fv[x] = 1.f;
 #pragma unroll
-        for (int e = 0; e < NC * VE; ++e) k[x][e] = v[x][e] = 0.f;
+        for (int e = 0; e < NE; ++e) k[x][e] = v[x][e] = 0.f;
         if (bits == 0) continue;
         const int j = __ffs(bits) - 1;
         bits &= bits - 1;
         ++taken;
-        const int32_t page = __shfl_sync(kFullMask, my_page, j), slot = __shfl_sync(kFullMask, my_slot, j);
-        const TC* kp = reinterpret_cast<const TC*>(a.c.K.data) + a.c.K.at(page, slot, h);
-        const TC* vp = reinterpret_cast<const TC*>(a.c.V.data) + a.c.V.at(page, slot, h);
+        const TC* kp = reinterpret_cast<const TC*>(a.c.K.data) + __shfl_sync(kFullMask, my_k, j);
+        const TC* vp = reinterpret_cast<const TC*>(a.c.V.data) + __shfl_sync(kFullMask, my_v, j);
 #pragma unroll
         for (int i = 0; i < NC; ++i)
           if (col(i) < d) {
@@ -605,92 +619,114 @@ __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArg
             for (int e = 0; e < VE; ++e) v[x][i * VE + e] = y[e];
           }
         if constexpr (IsByte<TC>::value) {
-          s[x] = a.c.K.scale[a.c.K.scale_at(page, slot, h)];
-          fv[x] = a.c.V.scale[a.c.V.scale_at(page, slot, h)];
-        } else {
-          s[x] = 1.f;
+          fk[x] = __shfl_sync(kFullMask, my_fk, j);
+          fv[x] = __shfl_sync(kFullMask, my_fv, j);
         }
       }
-      float top = M;
 #pragma unroll
-      for (int x = 0; x < KB; ++x) {
-        float y = 0.f;
+      for (int x = 0; x < KB; ++x)
 #pragma unroll
-        for (int e = 0; e < NC * VE; ++e) y = fmaf(q[e], IsByte<TC>::value ? k[x][e] * s[x] : k[x][e], y);
+        for (int r = 0; r < GR; ++r) {
+          s[x][r] = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) y += __shfl_xor_sync(kFullMask, y, o);
-        s[x] = x < taken ? y * a.scale_log2e : neg_inf();
-        top = max_nan(top, s[x]);
+          for (int e = 0; e < NE; ++e) s[x][r] = fmaf(q[r][e], IsByte<TC>::value ? k[x][e] * fk[x] : k[x][e], s[x][r]);
+        }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int x = 0; x < KB; ++x)
+#pragma unroll
+          for (int r = 0; r < GR; ++r) s[x][r] += __shfl_xor_sync(kFullMask, s[x][r], o);
+#pragma unroll
+      for (int r = 0; r < GR; ++r) {
+        float top = M[r];
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          s[x][r] = x < taken ? s[x][r] * a.scale_log2e : neg_inf();
+          top = max_nan(top, s[x][r]);
+        }
+        const float ref = top == neg_inf() ? 0.f : top, f = fast_exp2(M[r] - ref);
+        L[r] *= f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[r][e] *= f;
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          if (x >= taken) continue;
+          const float pr = fast_exp2(s[x][r] - ref);
+          L[r] += pr;
+#pragma unroll
+          for (int e = 0; e < NE; ++e) acc[r][e] = fmaf(pr, IsByte<TC>::value ? v[x][e] * fv[x] : v[x][e], acc[r][e]);
+        }
+        M[r] = top;
       }
-      const float ref = top == neg_inf() ? 0.f : top;
-      const float f = fast_exp2(M - ref);
-      L *= f;
-#pragma unroll
-      for (int e = 0; e < NC * VE; ++e) acc[e] *= f;
-#pragma unroll
-      for (int x = 0; x < KB; ++x) {
-        if (x >= taken) continue;
-        const float pr = fast_exp2(s[x] - ref);
-        L += pr;
-#pragma unroll
-        for (int e = 0; e < NC * VE; ++e) acc[e] = fmaf(pr, IsByte<TC>::value ? v[x][e] * fv[x] : v[x][e], acc[e]);
-      }
-      M = top;
     }
   }
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t tiles = a.tiles_of(len);
   if (tiles > 0) {
-    const int64_t x = (n - begin) * a.group + (hq - (int64_t)h * a.group);
-    const int64_t u = (int64_t)h * a.row_tiles(tokens) + x / a.row_tile;
+    const int64_t x = (n - begin) * a.group + g0;  // the rows lie in one unit (GR > 1: units hold whole tokens)
+    const int64_t u = (int64_t)h * a.row_tiles(tokens) + x / a.unit_rows;
     const int64_t chunk = a.cut[0], t = a.cut[1 + b] + u * tiles;
     const int64_t c0 = t / chunk, c1 = (t + tiles - 1) / chunk;
     for (int64_t c = c0; c <= c1; c += 32) {
       const int np = (int)(c1 - c + 1 < 32 ? c1 - c + 1 : 32);
       const int64_t row = a.partial_row(begin, tokens, h, x, c);
-      float2 ml = make_float2(neg_inf(), 0.f);
-      if (lane < np) ml = a.ml[row + (int64_t)lane * a.row_tile];
-      float top = ml.x;
+      float2 ml[GR];
+      float wgt[GR];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o));
-      top = max_nan(top, M);
-      const float ref = top == neg_inf() ? 0.f : top;
-      const float f = fast_exp2(M - ref), wgt = fast_exp2(ml.x - ref);
-      float sum = wgt * ml.y;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-      L = L * f + sum;
-#pragma unroll
-      for (int e = 0; e < NC * VE; ++e) acc[e] *= f;
-      constexpr int PB = NC * VE <= 8 ? 8 : 2;  // pieces whose rows are in flight together
-      for (int k0 = 0; k0 < np; k0 += PB) {
-        float y[PB][NC * VE];
-#pragma unroll
-        for (int k = 0; k < PB; ++k) {
-          const float* src = a.O + (row + (int64_t)(k0 + k) * a.row_tile) * a.d_pad;
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            float z[VE];
-#pragma unroll
-            for (int e = 0; e < VE; ++e) z[e] = 0.f;
-            if (k0 + k < np && col(i) < d) load_vec<float, VE>(src + col(i), z);
-#pragma unroll
-            for (int e = 0; e < VE; ++e) y[k][i * VE + e] = z[e];
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < PB; ++k) {
-          const float wk = __shfl_sync(kFullMask, wgt, (k0 + k) & 31);
-#pragma unroll
-          for (int e = 0; e < NC * VE; ++e) acc[e] = fmaf(k0 + k < np ? wk : 0.f, y[k][e], acc[e]);
-        }
+      for (int r = 0; r < GR; ++r) {
+        ml[r] = make_float2(neg_inf(), 0.f);
+        if (lane < np && r < rows) ml[r] = a.ml[row + (int64_t)lane * a.row_tile + r];
       }
-      M = top;
+#pragma unroll
+      for (int r = 0; r < GR; ++r) {
+        float top = ml[r].x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFullMask, top, o));
+        top = max_nan(top, M[r]);
+        const float ref = top == neg_inf() ? 0.f : top, f = fast_exp2(M[r] - ref);
+        wgt[r] = fast_exp2(ml[r].x - ref);
+        float sum = wgt[r] * ml[r].y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        L[r] = L[r] * f + sum;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) acc[r][e] *= f;
+        M[r] = top;
+      }
+      constexpr int PB = NE * GR <= 8 ? 8 : 2;  // pieces whose rows are in flight together
+      for (int k0 = 0; k0 < np; k0 += PB) {
+        float y[PB][GR][NE];
+#pragma unroll
+        for (int k = 0; k < PB; ++k)
+#pragma unroll
+          for (int r = 0; r < GR; ++r) {
+            const float* src = a.O + (row + (int64_t)(k0 + k) * a.row_tile + r) * a.d_pad;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+              float z[VE];
+#pragma unroll
+              for (int e = 0; e < VE; ++e) z[e] = 0.f;
+              if (k0 + k < np && r < rows && col(i) < d) load_vec<float, VE>(src + col(i), z);
+#pragma unroll
+              for (int e = 0; e < VE; ++e) y[k][r][i * VE + e] = z[e];
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < PB; ++k)
+#pragma unroll
+          for (int r = 0; r < GR; ++r) {
+            const float wk = __shfl_sync(kFullMask, wgt[r], (k0 + k) & 31);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) acc[r][e] = fmaf(k0 + k < np ? wk : 0.f, y[k][r][e], acc[r][e]);
+          }
+      }
     }
   }
-
-  finish_row<TQ, VE, NC>(a, g, n, hq, lane, M, L, acc);
+#pragma unroll
+  for (int r = 0; r < GR; ++r)
+    if (r < rows) finish_row<TQ, VE, NC>(a, g, n, hq + r, lane, M[r], L[r], acc[r]);
 }
 
 }  // namespace tree

@@ -47,10 +47,10 @@ int launch_context_any(const Call& a, bool vec, cudaStream_t st) {
 }
 
 // The merge kernel may start while the context kernel drains (programmatic dependent launch).
-template <class TQ, class TC, int VE, int NC>
+template <class TQ, class TC, int VE, int NC, int GR>
 int launch_merge(const Call& a, const MergeArgs& g, cudaStream_t st) {
-  const int64_t blocks = (a.n_rows * a.n_q_heads + 3) / 4;
-  if (blocks > kMost32) return SPFA_ERR_TOO_LARGE;
+  const int64_t blocks = (a.n_rows * a.c.n_heads * ((a.group + GR - 1) / GR) + 3) / 4;
+  if (blocks * 4 > kMost32) return SPFA_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(128);
@@ -60,21 +60,25 @@ int launch_merge(const Call& a, const MergeArgs& g, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, merge_kernel<TQ, TC, VE, NC>, a, g) != cudaSuccess) return SPFA_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, merge_kernel<TQ, TC, VE, NC, GR>, a, g) != cudaSuccess) return SPFA_ERR_LAUNCH;
   g_launches.fetch_add(1);
   return launch_status();
 }
 
+// From this many rows on (as many warps as 148 SMs hold) a warp merges four rows of a token: 53,248 rows of 4 heads a key head took
+// 104 us one by one.
+constexpr int64_t kMergeRows = 148 * 16;
 template <class TQ, class TC>
 int launch_merge_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
   const int d = a.c.d;
   if (vec) {
-    if (d <= 128) return launch_merge<TQ, TC, 4, 1>(a, g, st);
-    if (d <= 256) return launch_merge<TQ, TC, 4, 2>(a, g, st);
-    return launch_merge<TQ, TC, 4, 8>(a, g, st);
+    const bool four = a.group > 1 && (a.unit_rows % a.group == 0 || a.group % 4 == 0) && a.n_rows * a.n_q_heads > kMergeRows;
+    if (d <= 128) return four ? launch_merge<TQ, TC, 4, 1, 4>(a, g, st) : launch_merge<TQ, TC, 4, 1, 1>(a, g, st);
+    if (d <= 256) return launch_merge<TQ, TC, 4, 2, 1>(a, g, st);
+    return launch_merge<TQ, TC, 4, 8, 1>(a, g, st);
   }
-  if (d <= 128) return launch_merge<TQ, TC, 1, 4>(a, g, st);
-  return launch_merge<TQ, TC, 1, 32>(a, g, st);
+  if (d <= 128) return launch_merge<TQ, TC, 1, 4, 1>(a, g, st);
+  return launch_merge<TQ, TC, 1, 32, 1>(a, g, st);
 }
 
 template <class TQ, class TC, int R>
