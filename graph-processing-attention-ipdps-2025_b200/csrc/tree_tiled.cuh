@@ -171,7 +171,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   using TP = typename std::conditional<kQuant, __half, T>::type;  // operands of both products
   constexpr bool kMaySplit = !(kQuant && std::is_same<T, __nv_bfloat16>::value);
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // an offset: through an integer, every access below would be a generic one
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + P::kOffBar + 8u * i; };
   constexpr int B_KFULL = 0, B_KEMPTY = NS, B_VFULL = 2 * NS, B_VEMPTY = 3 * NS, B_CK = 4 * NS /* full [NC], empty [NC] */, B_CV = B_CK + 2 * NC, B_SREADY = B_CK + 4 * NC,
