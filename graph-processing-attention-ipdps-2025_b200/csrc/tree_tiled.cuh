@@ -488,10 +488,11 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     // =============================== softmax: one thread owns one query row ===============================
     // P = 2^(s - shift). A row's shift is the maximum it was last set at, less kLift, plus the exponent of the largest of V's scales
     // (8-bit caches, from 2^-80 on): it is set anew only when that outgrows it by kSlack. A float16 probability times its scale is
-    // below 2^(kLift + kSlack + 1) = 2^15 then, keeps 11 bits down to 2^-24 of its reference and steps of 2^-34 below, so that a
-    // million small ones lose less than 2^-15 of V's magnitude.
+    // below 2^(kLift + kSlack + 1) = 2^15 then, keeps 11 bits down to 2^-22 of its reference and steps of 2^-32 below, so that a
+    // million small ones lose less than 2^-13 of V's magnitude. Each new shift holds a warp up for some 2000 cycles, and the product
+    // with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
     constexpr bool kHalfP = std::is_same<TP, __half>::value;
-    constexpr float kSlack = kHalfP ? 4.f : 8.f, kLift = kHalfP ? 10.f : 0.f;
+    constexpr float kSlack = kHalfP ? 6.f : 8.f, kLift = kHalfP ? 8.f : 0.f;
     const uint64_t minus1 = pack2(-1.f, -1.f);
     constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included
     const int sub = warp / 4, tid = threadIdx.x % 128;
@@ -642,14 +643,14 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
             if (!warp_wait(bar(b_oready + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312)) return false;
             tc_fence_after();
-            uint32_t ob[8];
+            uint32_t ob[32];
 #pragma unroll 1
-            for (int c = 0; c < DP / 8; ++c) {
-              tmem_ld8(tO + c * 8, ob);
+            for (int c = 0; c < DP / 32; ++c) {
+              tmem_ld32(tO + c * 32, ob);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 8; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * f);
-              tmem_st8(tO + c * 8, ob);
+              for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * f);
+              tmem_st32(tO + c * 32, ob);
             }
           }
           shift = new_shift;
