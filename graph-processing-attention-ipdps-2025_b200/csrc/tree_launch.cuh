@@ -122,9 +122,9 @@ inline bool tiled_shape(const spfa_kv_cache* c) {
 }
 
 // Pages as (element, slot, head, page), fetched as boxes of a page's slots (at most kTiledKeys) x 128 bytes of 16-bit elements in the
-// swizzle of the tensor cores, or x `dp` codes of an 8-bit cache as they lie. Elements behind d and slots behind a page are zeros.
+// swizzle of the tensor cores, or x `bytes` codes of an 8-bit cache, as they lie or in that swizzle. Elements behind d and slots behind a page are zeros.
 template <class T>
-bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const int64_t* stride, int dp) {
+bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const int64_t* stride, int bytes, bool swizzle) {
   TensorMapEncodeTiledFn enc = tensor_map_encoder();
   if (!enc) return false;
   constexpr bool kByte = sizeof(T) == 1;
@@ -132,12 +132,12 @@ bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const in
   cuuint64_t strides[3] = {(cuuint64_t)stride[1] * sizeof(T), (cuuint64_t)stride[2] * sizeof(T), (cuuint64_t)stride[0] * sizeof(T)};
   for (int i = 0; i < 3; ++i)
     if (strides[i] == 0) strides[i] = 16;  // of a dimension of one element
-  const cuuint32_t box[4] = {kByte ? (cuuint32_t)dp : 64u, (cuuint32_t)(c->page_size < kTiledKeys ? c->page_size : kTiledKeys), 1u, 1u};
+  const cuuint32_t box[4] = {kByte ? (cuuint32_t)bytes : 64u, (cuuint32_t)(c->page_size < kTiledKeys ? c->page_size : kTiledKeys), 1u, 1u};
   const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUtensorMapDataType type = kByte ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                          : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
   return enc(tm, type, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             kByte ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -190,7 +190,8 @@ int launch_tiled(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool
     using P = PlanTree<DP, TC, NSUB>;
     int* err = tile_error_word();
     CUtensorMap tmK, tmV;
-    if (!err || !make_page_map<TC>(&tmK, c, c->K, c->K_stride, DP) || !make_page_map<TC>(&tmV, c, c->V, c->V_stride, DP))
+    if (!err || !make_page_map<TC>(&tmK, c, c->K, c->K_stride, P::kRawK ? 128 : DP, !P::kConvertK) ||
+        !make_page_map<TC>(&tmV, c, c->V, c->V_stride, DP, !P::kQuant))
       return SPFA_ERR_LAUNCH;
     context_tiled_kernel<DP, TQ, TC, NSUB><<<(unsigned)a.n_cta, P::kThreads, P::kDynSmem, st>>>(tmK, tmV, a, err);
     g_launches.fetch_add(1);

@@ -35,7 +35,7 @@ using namespace tile;
 // alone: K and V are fetched and converted once for both.
 template <int DP, class TC, int NSUB>
 struct PlanTree {
-  static constexpr bool kQuant = sizeof(TC) == 1;
+  static constexpr bool kQuant = sizeof(TC) == 1, kRawK = std::is_same<TC, e4m3>::value, kConvertK = kQuant && !kRawK;
   static constexpr int kSoftmaxWarps = 4 * NSUB, kAux = 4 * NSUB /* first of four warps */, kConvertFrom = kAux + 4;
   static constexpr int kConvert = kQuant ? 128 * NSUB : 0, kThreads = 128 * NSUB + 128 + kConvert, kCtasPerSm = 3 - NSUB;
   static constexpr int kRegsLaunch = NSUB == 1 ? (kQuant ? 80 : 128) : (kQuant ? 96 : 168);
@@ -44,14 +44,15 @@ struct PlanTree {
   static constexpr int kRegsNeeded = kRegsSoftmax * 128 * NSUB + kRegsAux * (kThreads - 128 * NSUB);
   static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
   static constexpr int TK = 64, kRows = 128 * NSUB, kChunks = DP / 64;
-  static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128, kQSub = kChunks * kQChunk, kQBytes = NSUB * kQSub;
+  static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128, kQSub = (kRawK ? 3 : kChunks) * kQChunk, kQBytes = NSUB * kQSub;
   static constexpr int kTile = kChunks * kKVChunk;               // a 16-bit tile of K or V
   static constexpr int kStage = kQuant ? TK * DP : kTile;        // a tile as it is fetched
+  static constexpr int kStageK = kRawK ? TK * 128 : kStage;      // K's, where it meets the tensor cores so: in their swizzle
   static constexpr int NS = (DP == 128 && NSUB == 1) ? 2 : 4;    // stages of K and of V
   static constexpr int NC = kQuant ? NSUB : 1;                   // converted tiles of K and of V
   static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
-  static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStage, kOffCK = kOffV + NS * kStage;
-  static constexpr int kOffCV = kOffCK + (kQuant ? NC * kTile : 0), kOffScale = kOffCV + (kQuant ? NC * kTile : 0);
+  static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStageK, kOffCK = kOffV + NS * kStage;
+  static constexpr int kOffCV = kOffCK + (kConvertK ? NC * kTile : 0), kOffScale = kOffCV + (kQuant ? NC * kTile : 0);
   static constexpr int kOffRow = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffRow + 128 * 8;
   static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 4 * NS + 4 * NC + 7 * NSUB;
   static constexpr int kOffCut = kOffBar + kNumBars * 8, kOffMisc = kOffCut + (int)sizeof(Cut);
@@ -110,6 +111,24 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void mma8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Two e4m3 numbers in the low half of a word, x in its lower byte; values beyond +-448 become those.
+__device__ __forceinline__ uint32_t e4m3_pair(float2 x) {
+  uint16_t y;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(x.y), "f"(x.x));
+  return y;
+}
+__device__ __forceinline__ float2 e4m3_floats(uint32_t x) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"((uint16_t)x));
+  return Half16<__half>::up(y);
+}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -167,7 +186,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                      int* __restrict__ err) {
   using P = PlanTree<DP, TC, NSUB>;
   constexpr int TK = P::TK, NS = P::NS, NC = P::NC;
-  constexpr bool kQuant = P::kQuant;
+  constexpr bool kQuant = P::kQuant, kRawK = P::kRawK, kConvertK = P::kConvertK;
+  constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // e4m3 numbers of an element of Q
   using TP = typename std::conditional<kQuant, __half, T>::type;  // operands of both products
   constexpr bool kMaySplit = !(kQuant && std::is_same<T, __nv_bfloat16>::value);
   extern __shared__ uint8_t smem_raw[];
@@ -188,7 +208,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(bar(B_KFULL + s), kQuant ? 33 : 1);
-      mbar_init(bar(B_KEMPTY + s), kQuant ? P::kConvert / 32 : NSUB);
+      mbar_init(bar(B_KEMPTY + s), kConvertK ? P::kConvert / 32 : NSUB);
       mbar_init(bar(B_VFULL + s), 1);
       mbar_init(bar(B_VEMPTY + s), kQuant ? P::kConvert / 32 : NSUB);
     }
@@ -216,7 +236,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmV)) : "memory");
   }
   if (!kQuant && a.tile_keys < TK) {  // rows that no box reaches: zero V, finite K
-    for (int x = threadIdx.x; x < 2 * NS * P::kStage / 16; x += P::kThreads) reinterpret_cast<uint4*>(smem + P::kOffK)[x] = make_uint4(0, 0, 0, 0);
+    for (int x = threadIdx.x; x < NS * (P::kStageK + P::kStage) / 16; x += P::kThreads) reinterpret_cast<uint4*>(smem + P::kOffK)[x] = make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   block_cut<P::kThreads>(a, cut);  // ends with a barrier
@@ -259,7 +279,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         key_page[x] = a.page_tiles ? 0 : min(key / ps, n_pages_tile - 1);
         key_slot[x] = key - key_page[x] * ps;
       }
-      const uint32_t tile_bytes = (uint32_t)(a.page_tiles ? TK : ps) * (kQuant ? DP : 128 * P::kChunks) * n_pages_tile;
+      const uint32_t stage = is_k ? P::kStageK : P::kStage, key_bytes = stage / TK;
+      const uint32_t tile_bytes = (uint32_t)(a.page_tiles ? TK : ps) * key_bytes * n_pages_tile;
       const uint32_t every = 0xffffffffu >> (32 - n_pages_tile);
       uint32_t jj = 0;
       bool ok = true;
@@ -312,7 +333,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             }
           }
           if (el) mbar_expect_tx(bar(full + st), tile_bytes);
-          uint32_t to = sbase + off + st * P::kStage;
+          uint32_t to = sbase + off + st * stage;
           for (int i = 0; i < n_pages_tile; ++i) {
             const int32_t page = __shfl_sync(kFullMask, cur, at + i);
             if (el) {
@@ -323,7 +344,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                 for (int c = 0; c < P::kChunks; ++c) tma_load_4d(to + c * P::kKVChunk, tm, c * 64, slot, w.h, page, bar(full + st));
               }
             }
-            to += ps * (kQuant ? DP : 128);
+            to += ps * (kQuant ? key_bytes : 128);
           }
           __syncwarp();
           if (a.page_tiles) {
@@ -342,6 +363,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       // =============================== MMA issuers: one for each row tile ===============================
       const int sub = NSUB == 2 && warp == P::kAux + 3 ? 1 : 0;
       const bool el = elect_one();
+      // (e4m3 has the code of float16 in the descriptor of kind::f8f6f4)
       constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
       const uint64_t qd = smem_desc(sbase + P::kOffQ + sub * P::kQSub, 16, 1024, kLayoutSw128);
       const uint32_t s_at = tmem + P::kColS + 2 * TK * sub, o_at = tmem + P::kColO + sub * DP;
@@ -353,7 +375,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const bool split = w.tokens * a.group <= 128;
         const bool idle = NSUB == 2 && sub == 1 && w.rows(a) <= 128;  // the unit has no second tile: only the stages are handed on
         auto k_ready = [&](uint32_t j) -> bool {
-          return warp_wait(bar(kQuant ? B_CK + j % NC : B_KFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 212);
+          return warp_wait(bar(kConvertK ? B_CK + j % NC : B_KFULL + j % NS), kConvertK ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 212);
         };
         auto v_ready = [&](uint32_t j) -> bool {
           return warp_wait(bar(kQuant ? B_CV + j % NC : B_VFULL + j % NS), kQuant ? (j / NC) & 1 : (j / NS) & 1, abort_flag, err, 214);
@@ -361,7 +383,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         if (idle) {
           for (int32_t t = 0; t < n && ok; ++t, ++jj) {
             ok = k_ready(jj);
-            if (ok && el) mbar_arrive(bar(kQuant ? B_CK + NC + jj % NC : B_KEMPTY + jj % NS));
+            if (ok && el) mbar_arrive(bar(kConvertK ? B_CK + NC + jj % NC : B_KEMPTY + jj % NS));
             ok = ok && v_ready(jj);
             if (ok && el) mbar_arrive(bar(kQuant ? B_CV + NC + jj % NC : B_VEMPTY + jj % NS));
           }
@@ -373,19 +395,27 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         auto issue_S = [&](int32_t t) -> bool {
           if (t >= n) return true;
           const uint32_t j = jj + (uint32_t)t, buf = (done + (uint32_t)t) & 1;
-          const int st = kQuant ? j % NC : j % NS;
+          const int st = kConvertK ? j % NC : j % NS;
           if (!k_ready(j)) return false;
           tc_fence_after();
-          const uint64_t kd = smem_desc(sbase + (kQuant ? P::kOffCK + st * P::kTile : P::kOffK + st * P::kStage), 16, 1024, kLayoutSw128);
+          const uint64_t kd = smem_desc(sbase + (kConvertK ? P::kOffCK + st * P::kTile : P::kOffK + st * P::kStageK), 16, 1024, kLayoutSw128);
           if (el) {
+            if constexpr (kRawK) {  // 32 elements (32 bytes) of the contraction per MMA, Q's terms one after the other
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {  // 16 elements (32 bytes) of the contraction per MMA
-              const int c = kk / 4, in = kk % 4 * 32;
-              mma16_ss(s_at + TK * buf, qd + (uint64_t)((c * P::kQChunk + in) >> 4), kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS,
-                       kk ? 1u : 0u);
+              for (int kk = 0; kk < kTerms * DP / 32; ++kk) {
+                const int term = kk / (DP / 32), in = kk % (DP / 32) * 32;
+                mma8_ss(s_at + TK * buf, qd + (uint64_t)((term * P::kQChunk + in) >> 4), kd + (uint64_t)(in >> 4), kIdescS, kk ? 1u : 0u);
+              }
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk) {  // 16 elements (32 bytes) of the contraction per MMA
+                const int c = kk / 4, in = kk % 4 * 32;
+                mma16_ss(s_at + TK * buf, qd + (uint64_t)((c * P::kQChunk + in) >> 4), kd + (uint64_t)((c * P::kKVChunk + in) >> 4), kIdescS,
+                         kk ? 1u : 0u);
+              }
             }
             tc_commit(bar(b_sready + buf));
-            tc_commit(bar(kQuant ? B_CK + NC + st : B_KEMPTY + st));
+            tc_commit(bar(kConvertK ? B_CK + NC + st : B_KEMPTY + st));
           }
           __syncwarp();
           return true;
@@ -436,7 +466,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     } else if (kQuant && warp >= P::kConvertFrom) {
       // =============================== the tiles of an 8-bit cache ===============================
       if constexpr (kQuant) {
-        // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1)
+        // K one tile ahead of V, as S runs ahead of P V: K0, K1 V0, K2 V1, ... V(n-1); or V alone
         constexpr int UPT = DP / 16, R = P::kConvert / UPT;  // 16-byte units of a row of codes, rows of one step
         const int tid = threadIdx.x - P::kConvertFrom * 32, r0 = tid / UPT, u = tid % UPT, ch = u / 4, s = ch & 1;
         // the two halves of d would meet in the same banks: the second one turns its pieces round
@@ -444,9 +474,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         uint32_t jj = 0;
         bool ok = true;
         while (ok && w.next(a)) {
-          for (int32_t step = 0; step < 2 * w.n && ok; ++step) {
-            const bool is_v = step > 0 && ((step & 1) == 0 || step == 2 * w.n - 1);
-            const int32_t t = step == 2 * w.n - 1 ? w.n - 1 : (step + 1) / 2 - (is_v ? 1 : 0);
+          const int32_t steps = kConvertK ? 2 * w.n : w.n;
+          for (int32_t step = 0; step < steps && ok; ++step) {
+            const bool is_v = !kConvertK || (step > 0 && ((step & 1) == 0 || step == steps - 1));
+            const int32_t t = !kConvertK ? step : step == steps - 1 ? w.n - 1 : (step + 1) / 2 - (is_v ? 1 : 0);
             const uint32_t j = jj + (uint32_t)t;
             const int st = j % NS, done = (is_v ? B_CV : B_CK) + j % NC;
             ok = warp_wait(bar((is_v ? B_VFULL : B_KFULL) + st), (j / NS) & 1, abort_flag, err, 412) &&
@@ -527,7 +558,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           }
         };
         [[maybe_unused]] float f = 1.f;
-        if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {  // times 2^(14 - exponent of the row's largest element)
+        if constexpr (kRawK || (kQuant && std::is_same<T, __nv_bfloat16>::value)) {  // times 2^(kTop - exponent of the row's largest element)
+          constexpr int kTop = kRawK ? 7 : 14;
           uint32_t top = 0;
 #pragma unroll 1
           for (int u = 0; u < DP / 8; u += 8) {
@@ -537,37 +569,68 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             for (int i = 0; i < 8; ++i) {
               const uint32_t x = __vmaxu2(__vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu),
                                           __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
-              top = max(top, max(x << 16, x & 0xffff0000u));
+              top = max(top, max(x & 0xffffu, x >> 16));
             }
           }
-          int e = (int)(top >> 23) - 127;
-          e = e > 127 ? 14 : (e < -100 ? -100 : e);  // not finite: as it is
-          f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-          sc *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+          int e = (int)(__float_as_uint(Half16<T>::up(top).x) >> 23) - 127;
+          const bool finite = e <= 127;
+          e = !finite ? kTop : (e < -100 ? -100 : e);
+          f = __uint_as_float((uint32_t)(127 + kTop - e) << 23);
+          sc *= __uint_as_float((uint32_t)(127 - kTop + e) << 23);
+          if (kRawK && !finite) f = __int_as_float(0x7fc00000);  // e4m3 has no infinities: the row is NaN
         }
 #pragma unroll 1
         for (int u = 0; u < DP / 8; u += 8) {
           uint4 q[8];
           eight(u, q);
+          uint8_t* dst = smem + P::kOffQ + sub * P::kQSub;
+          if constexpr (kRawK) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-            if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {
+            for (int i = 0; i < 8; i += 2) {
+              uint32_t codes[kTerms][4];
+              const uint32_t v[8] = {q[i].x, q[i].y, q[i].z, q[i].w, q[i + 1].x, q[i + 1].y, q[i + 1].z, q[i + 1].w};
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 y = Half16<__nv_bfloat16>::up(v[k]);
-                v[k] = Half16<__half>::down(y.x * f, y.y * f);
+              for (int k = 0; k < 8; k += 2) {
+                float2 x = Half16<T>::up(v[k]), y = Half16<T>::up(v[k + 1]);
+                x = make_float2(x.x * f, x.y * f);
+                y = make_float2(y.x * f, y.y * f);
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term) {
+                  const uint32_t lo = e4m3_pair(x), hi = e4m3_pair(y);
+                  codes[term][k / 2] = lo | (hi << 16);
+                  if (term < kTerms - 1) {  // what the rounding left: exact
+                    const float2 a2 = e4m3_floats(lo), b2 = e4m3_floats(hi);
+                    x = make_float2(x.x - a2.x, x.y - a2.y);
+                    y = make_float2(y.x - b2.x, y.y - b2.y);
+                  }
+                }
               }
-            }
-            if constexpr (Widen<TC>::kSwap) {
 #pragma unroll
-              for (int k = 0; k < 4; k += 2) {
-                const uint32_t x = v[k], y = v[k + 1];
-                v[k] = (x & 0xffffu) | (y << 16);
-                v[k + 1] = (x >> 16) | (y & 0xffff0000u);
-              }
+              for (int term = 0; term < kTerms; ++term)
+                *reinterpret_cast<uint4*>(dst + term * P::kQChunk + P::unit(tid, (u + i) / 2)) =
+                    make_uint4(codes[term][0], codes[term][1], codes[term][2], codes[term][3]);
             }
-            *reinterpret_cast<uint4*>(smem + P::kOffQ + sub * P::kQSub + (u / 8) * P::kQChunk + P::unit(tid, i)) = make_uint4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+              if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 y = Half16<__nv_bfloat16>::up(v[k]);
+                  v[k] = Half16<__half>::down(y.x * f, y.y * f);
+                }
+              }
+              if constexpr (Widen<TC>::kSwap) {
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                  const uint32_t x = v[k], y = v[k + 1];
+                  v[k] = (x & 0xffffu) | (y << 16);
+                  v[k + 1] = (x >> 16) | (y & 0xffff0000u);
+                }
+              }
+              *reinterpret_cast<uint4*>(dst + (u / 8) * P::kQChunk + P::unit(tid, i)) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
           }
         }
       }  // rows beyond the unit's keep what was there: no row's result depends on another's
