@@ -144,7 +144,7 @@ bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const in
 // As band16_usable: setmaxnreg.inc must be covered by what the launch allocates.
 template <int DP, class T, class TC, int NSUB>
 bool tiled_usable() {
-  using P = PlanTree<DP, TC, NSUB>;
+  using P = PlanTree<DP, T, TC, NSUB>;
   static std::atomic<int> cached[64];  // per device: 0 unknown, 1 usable, 2 not
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
@@ -187,7 +187,7 @@ int launch_tiled(const spfa_kv_cache* c, const Call& a, const MergeArgs& g, bool
   return with_tiled<TQ>(c, a.row_tile / 128, [&](auto* t, auto dp, auto n) -> int {
     using TC = typename std::remove_pointer<decltype(t)>::type;
     constexpr int DP = decltype(dp)::value, NSUB = decltype(n)::value;
-    using P = PlanTree<DP, TC, NSUB>;
+    using P = PlanTree<DP, TQ, TC, NSUB>;
     int* err = tile_error_word();
     CUtensorMap tmK, tmV;
     if (!err || !make_page_map<TC>(&tmK, c, c->K, c->K_stride, P::kRawK ? 128 : DP, !P::kConvertK) ||

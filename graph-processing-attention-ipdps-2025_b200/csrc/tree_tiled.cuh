@@ -33,9 +33,10 @@ using namespace tile;
 
 // NSUB: 128-row tiles that a CTA works on together, against the same K and V. One, and two CTAs share an SM; or two, and a CTA has it
 // alone: K and V are fetched and converted once for both.
-template <int DP, class TC, int NSUB>
+template <int DP, class T, class TC, int NSUB>
 struct PlanTree {
   static constexpr bool kQuant = sizeof(TC) == 1, kRawK = std::is_same<TC, e4m3>::value, kConvertK = kQuant && !kRawK;
+  static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // e4m3 numbers of an element of Q (kRawK)
   static constexpr int kSoftmaxWarps = 4 * NSUB, kAux = 4 * NSUB /* first of four warps */, kConvertFrom = kAux + 4;
   static constexpr int kConvert = kQuant ? 128 * NSUB : 0, kThreads = 128 * NSUB + 128 + kConvert, kCtasPerSm = 3 - NSUB;
   static constexpr int kRegsLaunch = NSUB == 1 ? (kQuant ? 80 : 128) : (kQuant ? 96 : 168);
@@ -44,11 +45,13 @@ struct PlanTree {
   static constexpr int kRegsNeeded = kRegsSoftmax * 128 * NSUB + kRegsAux * (kThreads - 128 * NSUB);
   static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
   static constexpr int TK = 64, kRows = 128 * NSUB, kChunks = DP / 64;
-  static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128, kQSub = (kRawK ? 3 : kChunks) * kQChunk, kQBytes = NSUB * kQSub;
+  // (two row tiles and e4m3: room for three terms with either type, 160 us against 170 with the stages right behind two)
+  static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128;
+  static constexpr int kQSub = (!kRawK ? kChunks : NSUB == 2 ? 3 : kTerms) * kQChunk, kQBytes = NSUB * kQSub;
   static constexpr int kTile = kChunks * kKVChunk;               // a 16-bit tile of K or V
   static constexpr int kStage = kQuant ? TK * DP : kTile;        // a tile as it is fetched
   static constexpr int kStageK = kRawK ? TK * 128 : kStage;      // K's, where it meets the tensor cores so: in their swizzle
-  static constexpr int NS = (DP == 128 && NSUB == 1) ? 2 : 4;    // stages of K and of V
+  static constexpr int NS = (DP == 64 || NSUB == 2) ? 4 : (kRawK && kTerms == 2) ? 3 : 2;  // stages of K and of V: what memory allows
   static constexpr int NC = kQuant ? NSUB : 1;                   // converted tiles of K and of V
   static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
   static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStageK, kOffCK = kOffV + NS * kStage;
@@ -129,6 +132,7 @@ __device__ __forceinline__ float2 e4m3_floats(uint32_t x) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"((uint16_t)x));
   return Half16<__half>::up(y);
 }
+
 __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -181,13 +185,13 @@ __device__ __noinline__ int infinity_of(const Call& a, int32_t b, int32_t h, int
 }
 
 template <int DP, class T, class TC, int NSUB>
-__global__ void __launch_bounds__(PlanTree<DP, TC, NSUB>::kThreads, PlanTree<DP, TC, NSUB>::kCtasPerSm)
+__global__ void __launch_bounds__(PlanTree<DP, T, TC, NSUB>::kThreads, PlanTree<DP, T, TC, NSUB>::kCtasPerSm)
 context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Call a,
                      int* __restrict__ err) {
-  using P = PlanTree<DP, TC, NSUB>;
+  using P = PlanTree<DP, T, TC, NSUB>;
   constexpr int TK = P::TK, NS = P::NS, NC = P::NC;
   constexpr bool kQuant = P::kQuant, kRawK = P::kRawK, kConvertK = P::kConvertK;
-  constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // e4m3 numbers of an element of Q
+  constexpr int kTerms = P::kTerms;
   using TP = typename std::conditional<kQuant, __half, T>::type;  // operands of both products
   constexpr bool kMaySplit = !(kQuant && std::is_same<T, __nv_bfloat16>::value);
   extern __shared__ uint8_t smem_raw[];
@@ -298,11 +302,15 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           nxt = pages_at(more);
         };
         turn(base + 32);
-        for (int32_t t = 0; t < w.n; ++t, ++jj) {
-          if (first >= base + 32) {
-            base += 32;
-            turn(base + 32);
+        [[maybe_unused]] const float *ks[2], *vs[2];  // scales of this lane's two keys, on page 0
+        if (kQuant && is_k) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            ks[x] = a.c.K.scale + a.c.K.scale_at(0, key_slot[x], w.h);
+            vs[x] = a.c.V.scale + a.c.V.scale_at(0, key_slot[x], w.h);
           }
+        }
+        for (int32_t t = 0; t < w.n; ++t, ++jj) {
           const int st = jj % NS;
           ok = warp_wait(bar(empty + st), ((jj / NS) & 1) ^ 1u, abort_flag, err, is_k ? 111 : 112);
           if (!ok) break;
@@ -316,16 +324,16 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             }
             if (el) ring_mask[jj % P::kRing] = mask;
             if constexpr (kQuant) {
-              float* dst = ring_scale + (jj % P::kRing) * 2 * TK;
+              const uint32_t dst = sbase + P::kOffScale + ((jj % P::kRing) * 2 * TK + lane) * 4;
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                const int key = lane + 32 * x;
-                const int64_t page = __shfl_sync(kFullMask, cur, at + key_page[x]);
-                if ((mask >> key) & 1) {
-                  cp_async4(smem_u32(dst + key), a.c.K.scale + a.c.K.scale_at(page, slot + key_slot[x], w.h));
-                  cp_async4(smem_u32(dst + TK + key), a.c.V.scale + a.c.V.scale_at(page, slot + key_slot[x], w.h));
+                const int32_t page = __shfl_sync(kFullMask, cur, at + key_page[x]);
+                if (lane + 32 * x < n && page < a.c.n_pages) {
+                  cp_async4(dst + 128 * x, ks[x] + page * a.c.K.s_stride[0] + slot * a.c.K.s_stride[1]);
+                  cp_async4(dst + 128 * x + TK * 4, vs[x] + page * a.c.V.s_stride[0] + slot * a.c.V.s_stride[1]);
                 } else {
-                  dst[key] = dst[TK + key] = 0.f;
+                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128 * x), "f"(0.f) : "memory");
+                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128 * x + TK * 4), "f"(0.f) : "memory");
                 }
               }
               cp_async_arrive(bar(B_KFULL + st));
@@ -355,6 +363,10 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             }
           } else {
             first += n_pages_tile;
+          }
+          if (first >= base + 32) {
+            base += 32;
+            turn(base + 32);
           }
         }
       }
