@@ -67,7 +67,6 @@ struct Cut {  // what block_cut leaves in shared memory
   int64_t first, last;  // this CTA's key tiles in the list
   int64_t start;        // first tile of sequence b
   int32_t b;
-  int32_t warp_sum_at;  // (padding)
   int64_t warp_sum[32];
 };
 
@@ -552,7 +551,10 @@ __global__ void __launch_bounds__(128) merge_kernel(const Call a, const MergeArg
   const int rows = GR == 1 ? 1 : min(GR, a.group - g0);
   const int32_t hq = h * a.group + g0;
   const int32_t b = n < a.n_rows ? sequence_of(a.cu_rows, a.c.n_seq, n) : -1;
-  if (b < 0) return;
+  if (b < 0) {  // the grid ends behind the context kernel's end, whatever its rows are
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   int64_t begin, end;
   rows_of(a.cu_rows, b, a.n_rows, begin, end);
   const int64_t tokens = end - begin, len = a.c.len_of(b);

@@ -436,3 +436,47 @@ def test_every_code_is_taken_as_its_value(pkg, cache, dtype):
         for tag, (m, l, O) in both_paths(pkg, c, Q, cu, none):
             bad = torch.tensor([[False, False, True, False]])
             assert torch.equal(torch.isnan(m.cpu()), bad) and torch.equal(torch.isnan(O.cpu()).all(-1), bad), tag
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "native"), ("bf16", "native"), ("f16", "int8"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 2), (6, 2), (12, 3), (5, 1), (12, 2), (14, 2), (18, 2), (20, 1), (67, 1), (130, 1)])
+def test_many_rows_are_merged_together(pkg, Hq, Hkv, dtype, cache):
+    """Calls of many rows merge several query heads at a time: groups that four divides and others, groups that no row tile divides,
+    units that end inside a token; twice, on the state that the first call left."""
+    tokens = 2400 // Hq + 1  # more rows than the machine holds warps
+    rows = [tokens // 2, 0, 1, tokens - tokens // 2]
+    c, Q, cu, mask = problem(dtype, cache, [70, 9, 0, 33], rows, Hq, Hkv, 64, 16, "hnd", seed=Hq, width=40)
+    want, bound, written = tree_reference(c, Q, cu, mask)
+    got = run(pkg, c, Q, cu, mask)
+    check_tree(got, want, bound, written, "first")
+    given = tuple(x.double().cpu().numpy() for x in got)
+    want, bound, _ = tree_reference(c, Q, cu, mask, state=given)
+    check_tree(run(pkg, c, Q, cu, mask, state=got), want, bound, written, "again")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_query_rows_of_a_wide_range_over_e4m3(pkg, dtype, rows):
+    """Q meets an e4m3 cache as two (bfloat16) or three (float16) e4m3 numbers an element, the row's largest between 2^7 and 2^8 and
+    the smallest step 2^-9: what falls below half of that, at most 2^-17 of the row's largest, is lost. A score is off by
+    dq = 2^-17 max|q| sum|k| / sqrt(d) then, a probability by 2 dq, O by 4 dq max|v|. Rows that are not finite are NaN."""
+    c, Q, cu, mask = problem(dtype, "e4m3", [700], [rows], 8, 2, 128, 16, seed=rows)
+    g = torch.Generator().manual_seed(1)
+    low = -12 if dtype == "f16" else -24
+    Q = Q * torch.exp2(torch.randint(low, 1, Q.shape, generator=g).float()).to(Q.dtype)
+    want, bound, written = tree_reference(c, Q, cu, mask)
+    k = np.abs(c.dense("K", 0, range(700 + rows))[0]).sum(-1).max()
+    v = np.abs(c.dense("V", 0, range(700 + rows))[0]).max()
+    dq = 2.0 ** -17 * np.abs(Q.double().numpy()).max(-1) * k / np.sqrt(128)
+    bound = (bound[0] + dq, bound[1] + 2 * dq * want[1], bound[2] + 4 * (dq * v)[..., None])
+    pkg.capi.set_path(pkg.capi.PATH_TILED)
+    try:
+        check_tree(run(pkg, c, Q, cu, mask), want, bound, written)
+        Q[1, 2, 5], Q[2, 1, 0] = float("inf"), float("nan")
+        m, l, O = run(pkg, c, Q, cu, mask)
+        assert torch.isnan(O[1, 2]).all() and torch.isnan(O[2, 1]).all()
+        others = torch.ones(rows, 8, dtype=torch.bool)
+        others[1, 2] = others[2, 1] = False
+        assert torch.isfinite(O[others.cuda()]).all() and torch.isfinite(m[others.cuda()]).all()
+    finally:
+        pkg.capi.set_path(pkg.capi.PATH_AUTO)
