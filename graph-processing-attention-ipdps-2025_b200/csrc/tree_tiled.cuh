@@ -12,16 +12,28 @@
 //              bytes of d. Pages that do not exist are fetched from behind the last one, where the copy engine fills with zeros.
 //   warp 5     MMA issuer
 //   warp 6     TMA producer of V
-//   warps 8-11 (8-bit caches) the conversion of each tile to 16 bits
+//   warps 8-11 (8-bit caches) the conversion of V, and of int8 K, to 16 bits
+//   With two row tiles: warps 0-7 softmax, 8-11 the roles of 4-7 (11 the second tile's MMA issuer), 12-19 the conversion.
 // A unit of at most 64 (32) rows has them two (four) times in Q: each copy takes half (a quarter) of every tile's columns, so that all
 // four softmax warps work, and the copies are added up at the end of the piece.
-// An 8-bit tile meets the tensor cores as float16 numbers that equal its codes (11 bits hold e4m3 and int8). The rows' scales stay in
-// fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the largest of them in. bfloat16 Q rows become float16 times a power of two: none of their 8 bits is
-// lost above 2^-29 of the row's largest element, and below nothing that a float32 sum of the products would show.
+// An int8 tile meets the tensor cores as float16 numbers that equal its codes, as V of e4m3 does. K of e4m3 meets them as it lies, in the
+// products of 8-bit numbers, and Q as e4m3 terms, each the rounding of what the terms before left: a row is first multiplied by a power
+// of two that brings its largest element to [2^7, 2^8); two terms are a bfloat16 element then, down to 2^-9 of that, three a float16
+// element down to 2^-6, and what is smaller is held to 2^-17 of the largest: that is the order of a sum of float32 products. (Without
+// K's conversion, which passes the tile through shared memory twice: 437 -> 370 us, e4m3 call below.) bfloat16 Q over int8 becomes
+// float16 times such a power: none of its 8 bits is lost above 2^-29 of the row's largest element.
+// The rows' scales stay in fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the
+// largest of them in.
 // P is rounded to 16 bits. Where that alone would be as large as the rounding of the result (all but 8-bit caches under bfloat16 Q),
 // units of a single row tile carry a second 16-bit term, the rounding's remainder: they wait for memory, and the second product is
 // hidden. Units with more row tiles are bound by arithmetic and rows enough that the error stays at its mean, sqrt(2) of the
 // result's own rounding.
+//
+// What bounds it, on 32 sequences of up to 32768 keys, 8 tokens, 4 heads a key head (32 rows a unit), d = 128: a bfloat16 cache memory,
+// 461 us, 5.9 TB/s; e4m3 370 us, 3.8 TB/s, and int8 500 us, 2.8 TB/s, shared memory: V's (int8: K's too) way through the converting warps,
+// Q and the converted tiles on theirs to the tensor cores add up to its 128 bytes a cycle. Units of 256 rows are bound by the softmax
+// warps, each of which owns a row of 64 scores a tile: 403 us, 700 TFLOP/s for 64 tokens over 16384 bfloat16 keys, 175 us and 436 TFLOP/s
+// for 64 tokens of 8 heads over 16384 int8 keys under float16 Q.
 #pragma once
 #include "tile_kernels_16.cuh"
 #include "tree_kernels.cuh"
@@ -62,7 +74,7 @@ struct PlanTree {
   static constexpr int kDynSmem = kOffMisc + 16 + 1024;
   static_assert(kCtasPerSm * (kDynSmem + 1024) <= 228 * 1024, "shared memory of an SM");
   // The producer writes the ring's entry of a tile once the tile NS before has left its stage, which is behind the softmax of the
-  // tile two (8-bit: two and NC) before that one.
+  // tile two (K converted: two and NC) before that one.
   static_assert(NS + 2 + NC <= kRing, "ring entries are written again only after they were read");
   static constexpr int kColS = 0, kColO = NSUB * 2 * TK, kTmemCols = 256 * NSUB;
   static_assert(kColO + NSUB * DP <= kTmemCols, "S buffers and the O accumulators exceed the TMEM allocation");
