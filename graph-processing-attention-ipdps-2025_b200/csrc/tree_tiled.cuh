@@ -574,27 +574,21 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const int32_t xr = w.row0 + sub * 128 + row, t = xr / a.group;
         const T* src = reinterpret_cast<const T*>(a.Q) + (int64_t)(w.begin + t) * a.q_stride[0] +
                        ((int64_t)w.h * a.group + (xr - t * a.group)) * a.q_stride[1];
-        auto eight = [&](int u0, uint4 (&q)[8]) {  // eight 16-byte units, all in flight together
+        uint4 q[DP / 8];  // all in flight together
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            q[i] = make_uint4(0, 0, 0, 0);
-            if ((u0 + i) * 8 < a.c.d) q[i] = __ldg(reinterpret_cast<const uint4*>(src) + u0 + i);
-          }
-        };
+        for (int i = 0; i < DP / 8; ++i) {
+          q[i] = make_uint4(0, 0, 0, 0);
+          if (i * 8 < a.c.d) q[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        }
         [[maybe_unused]] float f = 1.f;
         if constexpr (kRawK || (kQuant && std::is_same<T, __nv_bfloat16>::value)) {  // times 2^(kTop - exponent of the row's largest element)
           constexpr int kTop = kRawK ? 7 : 14;
           uint32_t top = 0;
-#pragma unroll 1
-          for (int u = 0; u < DP / 8; u += 8) {
-            uint4 q[8];
-            eight(u, q);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t x = __vmaxu2(__vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu),
-                                          __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
-              top = max(top, max(x & 0xffffu, x >> 16));
-            }
+          for (int i = 0; i < DP / 8; ++i) {
+            const uint32_t x = __vmaxu2(__vmaxu2(q[i].x & 0x7fff7fffu, q[i].y & 0x7fff7fffu),
+                                        __vmaxu2(q[i].z & 0x7fff7fffu, q[i].w & 0x7fff7fffu));
+            top = max(top, max(x & 0xffffu, x >> 16));
           }
           int e = (int)(__float_as_uint(Half16<T>::up(top).x) >> 23) - 127;
           const bool finite = e <= 127;
@@ -603,58 +597,53 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           sc *= __uint_as_float((uint32_t)(127 - kTop + e) << 23);
           if (kRawK && !finite) f = __int_as_float(0x7fc00000);  // e4m3 has no infinities: the row is NaN
         }
-#pragma unroll 1
-        for (int u = 0; u < DP / 8; u += 8) {
-          uint4 q[8];
-          eight(u, q);
-          uint8_t* dst = smem + P::kOffQ + sub * P::kQSub;
-          if constexpr (kRawK) {
+        uint8_t* dst = smem + P::kOffQ + sub * P::kQSub;
+        if constexpr (kRawK) {
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-              uint32_t codes[kTerms][4];
-              const uint32_t v[8] = {q[i].x, q[i].y, q[i].z, q[i].w, q[i + 1].x, q[i + 1].y, q[i + 1].z, q[i + 1].w};
+          for (int i = 0; i < DP / 8; i += 2) {
+            uint32_t codes[kTerms][4];
+            const uint32_t v[8] = {q[i].x, q[i].y, q[i].z, q[i].w, q[i + 1].x, q[i + 1].y, q[i + 1].z, q[i + 1].w};
 #pragma unroll
-              for (int k = 0; k < 8; k += 2) {
-                float2 x = Half16<T>::up(v[k]), y = Half16<T>::up(v[k + 1]);
-                x = make_float2(x.x * f, x.y * f);
-                y = make_float2(y.x * f, y.y * f);
+            for (int k = 0; k < 8; k += 2) {
+              float2 x = Half16<T>::up(v[k]), y = Half16<T>::up(v[k + 1]);
+              x = make_float2(x.x * f, x.y * f);
+              y = make_float2(y.x * f, y.y * f);
 #pragma unroll
-                for (int term = 0; term < kTerms; ++term) {
-                  const uint32_t lo = e4m3_pair(x), hi = e4m3_pair(y);
-                  codes[term][k / 2] = lo | (hi << 16);
-                  if (term < kTerms - 1) {  // what the rounding left: exact
-                    const float2 a2 = e4m3_floats(lo), b2 = e4m3_floats(hi);
-                    x = make_float2(x.x - a2.x, x.y - a2.y);
-                    y = make_float2(y.x - b2.x, y.y - b2.y);
-                  }
+              for (int term = 0; term < kTerms; ++term) {
+                const uint32_t lo = e4m3_pair(x), hi = e4m3_pair(y);
+                codes[term][k / 2] = lo | (hi << 16);
+                if (term < kTerms - 1) {  // what the rounding left: exact
+                  const float2 a2 = e4m3_floats(lo), b2 = e4m3_floats(hi);
+                  x = make_float2(x.x - a2.x, x.y - a2.y);
+                  y = make_float2(y.x - b2.x, y.y - b2.y);
                 }
               }
-#pragma unroll
-              for (int term = 0; term < kTerms; ++term)
-                *reinterpret_cast<uint4*>(dst + term * P::kQChunk + P::unit(tid, (u + i) / 2)) =
-                    make_uint4(codes[term][0], codes[term][1], codes[term][2], codes[term][3]);
             }
-          } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-              if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {
+            for (int term = 0; term < kTerms; ++term)
+              *reinterpret_cast<uint4*>(dst + term * P::kQChunk + P::unit(tid, i / 2)) =
+                  make_uint4(codes[term][0], codes[term][1], codes[term][2], codes[term][3]);
+          }
+        } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 y = Half16<__nv_bfloat16>::up(v[k]);
-                  v[k] = Half16<__half>::down(y.x * f, y.y * f);
-                }
+          for (int i = 0; i < DP / 8; ++i) {
+            uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+            if constexpr (kQuant && std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 y = Half16<__nv_bfloat16>::up(v[k]);
+                v[k] = Half16<__half>::down(y.x * f, y.y * f);
               }
-              if constexpr (Widen<TC>::kSwap) {
-#pragma unroll
-                for (int k = 0; k < 4; k += 2) {
-                  const uint32_t x = v[k], y = v[k + 1];
-                  v[k] = (x & 0xffffu) | (y << 16);
-                  v[k + 1] = (x >> 16) | (y & 0xffff0000u);
-                }
-              }
-              *reinterpret_cast<uint4*>(dst + (u / 8) * P::kQChunk + P::unit(tid, i)) = make_uint4(v[0], v[1], v[2], v[3]);
             }
+            if constexpr (Widen<TC>::kSwap) {
+#pragma unroll
+              for (int k = 0; k < 4; k += 2) {
+                const uint32_t x = v[k], y = v[k + 1];
+                v[k] = (x & 0xffffu) | (y << 16);
+                v[k + 1] = (x >> 16) | (y & 0xffff0000u);
+              }
+            }
+            *reinterpret_cast<uint4*>(dst + i / 8 * P::kQChunk + P::unit(tid, i % 8)) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       }  // rows beyond the unit's keep what was there: no row's result depends on another's
@@ -817,6 +806,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       }
       const int64_t out = a.partial_row(w.begin, w.tokens, w.h, w.row0 + sub * 128, blockIdx.x);
       if (mine && copy == 0) a.ml[out + row] = make_float2(m, l);
+      constexpr int kAtOnce = P::kQSub / (128 * 128) >= 2 && DP >= 64 ? 2 : 1;  // pieces of 32 columns that find room where Q was
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         uint32_t ob[32];
@@ -854,19 +844,21 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               if (c * 32 + e < a.d_pad) *reinterpret_cast<uint4*>(dst + e) = four(e);
           }
           __syncwarp();
-        } else {  // the copies are added up where Q was, 32 columns at a time
+        } else {  // the copies are added up where Q was
+          const int part = c % kAtOnce;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + P::unit(tid, e / 4)) = four(e);
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + part * P::kQChunk + P::unit(tid, e / 4)) = four(e);
+          if (part < kAtOnce - 1) continue;
           group_sync();
-          for (int x = tid; x < rows * 8; x += 128) {
-            const int r = x / 8, u = x % 8;
+          for (int x = tid; x < rows * 8 * kAtOnce; x += 128) {
+            const int r = x / (8 * kAtOnce), u = x % (8 * kAtOnce), col = (c - part) * 32 + u * 4;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < kCopies; ++k) {
-              const float4 z = *reinterpret_cast<const float4*>(smem + P::kOffQ + P::unit(k * kBlock + r, u));
+              const float4 z = *reinterpret_cast<const float4*>(smem + P::kOffQ + u / 8 * P::kQChunk + P::unit(k * kBlock + r, u % 8));
               y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
             }
-            if (c * 32 + u * 4 < a.d_pad) *reinterpret_cast<float4*>(a.O + (out + r) * a.d_pad + c * 32 + u * 4) = y;
+            if (col < a.d_pad) *reinterpret_cast<float4*>(a.O + (out + r) * a.d_pad + col) = y;
           }
           group_sync();
         }
