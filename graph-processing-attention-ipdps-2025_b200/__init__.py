@@ -1,11 +1,12 @@
 """B200 (sm_100a) sparse FlashAttention forward operators.
 
-Drop-in for the six operators of KLab-AI3/Graph-Processing-Attention-IPDPS-2025. Three layers:
+Drop-in for the six operators of KLab-AI3/Graph-Processing-Attention-IPDPS-2025; and paged key / value caches (append, read,
+keep) with the attention of drafted token trees over them. Three layers:
 
 * ``lib/libspfa_b200.so`` -- the C-ABI library (include/spfa_b200.h) with the hand-written CUDA kernels;
 * ``lib/spfa_<mask>.*.so`` -- six torch-extension modules with the reference's module names and
   ``forward`` signatures (``import spfa_csr`` etc. once :func:`add_bindings_to_path` ran, or via
-  :func:`binding`);
+  :func:`binding`), and three with operators that it has not: ``spfa_bigbird``, ``spfa_cache``, ``spfa_tree``;
 * :mod:`capi` -- a ctypes view of the C ABI that takes torch CUDA tensors (row-range sharding lives
   here, it has no counterpart in the reference's single-GPU API);
 * :mod:`hostio` -- forward calls on pinned HOST buffers for the banded masks, with the copies and the row-range
@@ -38,7 +39,7 @@ def add_bindings_to_path() -> str:
 
 
 def binding(name: str):
-    """Import one of the six torch-extension modules by the reference's module name."""
+    """Import one of the torch-extension modules by its name (of the six operators: the reference's)."""
     if name not in MODULES:
         raise ValueError(f"unknown module {name!r}; expected one of {MODULES}")
     import torch  # noqa: F401  (the extensions link against libtorch)

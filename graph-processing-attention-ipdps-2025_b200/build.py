@@ -1,11 +1,11 @@
-"""In-tree build of the sm_100a library and the six torch-extension bindings.
+"""In-tree build of the sm_100a library and the torch-extension bindings.
 
     python build.py            # build what is out of date
     python build.py --force    # rebuild everything
 
 Outputs (all under lib/, git-ignored):
     libspfa_b200.so                    C-ABI library (nvcc, -gencode arch=compute_100a,code=sm_100a)
-    spfa_csr.*.so ... (six modules)    pybind/torch bindings, linked against libspfa_b200.so via $ORIGIN
+    spfa_csr.*.so ... (nine modules)   pybind/torch bindings, linked against libspfa_b200.so via $ORIGIN
 
 Only sm_100a is targeted. There is no other backend and no CPU fallback.
 """

@@ -426,10 +426,19 @@ int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t wid
  * see no key get m = -inf, l = 0, O = 0. With first = 0 such rows are left as they are, and an incoming row with l = 0 is empty:
  * its O does not count. O may be Q itself (same strides); otherwise nothing that is written may overlap anything that is read.
  *
- * dtype: type of Q and O (equal to the cache's where that holds its values as they are). float32 calls compute in float32.
- * 16-bit calls run the committed positions on the tensor cores where d is at most 128, rows are 16-byte aligned (d a multiple
- * of 8, of an 8-bit cache 16) and pages hold a multiple of 8 positions or at least 64; their probabilities enter the product with
- * V as one 16-bit number each (bfloat16 where the cache is 8-bit or bfloat16). Everything else is computed in float32.
+ * dtype: type of Q and O (equal to the cache's where that holds its values as they are). float32 calls compute in float32, and so
+ * do calls of a few rows over short page lists (one launch). Other 16-bit calls run the committed positions on the tensor cores
+ * where d is at most 128, rows are 16-byte aligned (d a multiple of 8, of an 8-bit cache 16) and pages hold a multiple of 8
+ * positions or at least 64; with SPFA_PATH_TILED they do or return SPFA_ERR_BAD_ARG, with SPFA_PATH_GATHER they do not. There
+ *   - probabilities enter the product with V as 16-bit numbers, float16 over an 8-bit cache, else Q's type: two, the rounding and
+ *     what it left, where a sequence has at most 128 rows for a key head (tokens x query heads), except over an 8-bit cache under
+ *     bfloat16 Q; else one;
+ *   - over an e4m3 cache, Q's elements keep their value down to 2^-9 (bfloat16) or 2^-6 (float16) of the largest in their row, and
+ *     smaller ones are held to 2^-17 of it; a row of Q that is not finite gives NaN;
+ *   - over an int8 cache, bfloat16 elements of Q keep theirs down to 2^-29 of the largest in their row;
+ *   - scales of an 8-bit cache are not negative and finite, at most 2^96 of K and 2^100 of V, or NaN: a NaN scale of K or V makes
+ *     the rows that see it NaN. V below 2^-71 throughout a sequence loses bits, down to zeros.
+ * Everything else is computed in float32.
  * The workspace needs spfa_tree_workspace_bytes of the same cache, n_rows and n_q_heads. */
 size_t spfa_tree_workspace_bytes(const spfa_kv_cache* cache, int dtype, int64_t n_rows, int64_t n_q_heads);
 int spfa_tree_forward(const spfa_kv_cache* cache, int dtype, const void* Q, const int64_t* Q_stride, const int32_t* cu_rows,
@@ -467,8 +476,9 @@ int spfa_mask_fill(int kind, int64_t L, int64_t p0, int64_t p1,
 
 /* Reads and clears the error word of the tiled kernels on the current device. Synchronises the device.
  * 0 = no error; a positive code names the bounded wait that gave up (1xx TMA producer, 2xx MMA issuer,
- * 3xx softmax group); -1 = the CUDA runtime reported an error. No counterpart in the reference, whose
- * launches are never checked (sp_flatt_csr_kernel.cu:271). */
+ * 3xx softmax group, 41x conversion of 8-bit tiles) or 401, a stored plan of other sizes; -1 = the CUDA runtime
+ * reported an error. No counterpart in the reference, whose launches are never checked
+ * (sp_flatt_csr_kernel.cu:271). */
 int spfa_last_device_error(void);
 
 /* Diagnostics: exercises the time limit of the device-side waits without touching any data. Launches a
