@@ -17,10 +17,11 @@
 // A unit of at most 64 (32) rows has them two (four) times in Q: each copy takes half (a quarter) of every tile's columns, so that all
 // four softmax warps work, and the copies are added up at the end of the piece.
 // An int8 tile meets the tensor cores as float16 numbers that equal its codes, as V of e4m3 does. K of e4m3 meets them as it lies, in the
-// products of 8-bit numbers, and Q as e4m3 terms, each the rounding of what the terms before left: a row is first multiplied by a power
-// of two that brings its largest element to [2^7, 2^8); two terms are a bfloat16 element then, down to 2^-9 of that, three a float16
-// element down to 2^-6, and what is smaller is held to 2^-17 of the largest: that is the order of a sum of float32 products. (Without
-// K's conversion, which passes the tile through shared memory twice: 437 -> 370 us, e4m3 call below.) bfloat16 Q over int8 becomes
+// products of 8-bit numbers, and Q as terms of 8 bits, each the rounding of what the terms before left, the first e4m3, the others e5m2. A
+// row is first multiplied by a power of two that brings its largest element to [2^7, 2^8): two terms are a bfloat16 element then, and
+// three a float16 element, exactly, down to 2^-13 of the largest (2^-6, where e4m3's subnormal numbers begin), and smaller ones are held to
+// 2^-21 or 2^-24 of it. (e4m3 alone, which ends at 2^-9, showed in l: 9e-7 of it, float32 sums 4e-7.) Without K's conversion, which
+// passes the tile through shared memory twice: 437 -> 370 us, e4m3 call below. bfloat16 Q over int8 becomes
 // float16 times such a power: none of its 8 bits is lost above 2^-29 of the row's largest element.
 // The rows' scales stay in fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the
 // largest of them in.
@@ -48,7 +49,7 @@ using namespace tile;
 template <int DP, class T, class TC, int NSUB>
 struct PlanTree {
   static constexpr bool kQuant = sizeof(TC) == 1, kRawK = std::is_same<TC, e4m3>::value, kConvertK = kQuant && !kRawK;
-  static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // e4m3 numbers of an element of Q (kRawK)
+  static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // 8-bit numbers of an element of Q (kRawK)
   static constexpr int kSoftmaxWarps = 4 * NSUB, kAux = 4 * NSUB /* first of four warps */, kConvertFrom = kAux + 4;
   static constexpr int kConvert = kQuant ? 128 * NSUB : 0, kThreads = 128 * NSUB + 128 + kConvert, kCtasPerSm = 3 - NSUB;
   static constexpr int kRegsLaunch = NSUB == 1 ? (kQuant ? 80 : 128) : (kQuant ? 96 : 168);
@@ -133,16 +134,22 @@ __device__ __forceinline__ void mma8_ss(uint32_t d_tmem, uint64_t a_desc, uint64
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
       : "memory");
 }
-// Two e4m3 numbers in the low half of a word, x in its lower byte; values beyond +-448 become those.
-__device__ __forceinline__ uint32_t e4m3_pair(float2 x) {
+// Two 8-bit numbers of a term in the low half of a word, x's in its lower byte, and what their rounding leaves of x (exact).
+// The first term is e4m3, the others e5m2: its 3 bits hold what 4 bits leave of 8, and its range goes on down to 2^-16.
+template <bool kFirst>
+__device__ __forceinline__ uint32_t take_term(float2& x) {
   uint16_t y;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(x.y), "f"(x.x));
+  uint32_t back;
+  if constexpr (kFirst) {
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(y));
+  } else {
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(y) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(back) : "h"(y));
+  }
+  const float2 held = Half16<__half>::up(back);
+  x = make_float2(x.x - held.x, x.y - held.y);
   return y;
-}
-__device__ __forceinline__ float2 e4m3_floats(uint32_t x) {
-  uint32_t y;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"((uint16_t)x));
-  return Half16<__half>::up(y);
 }
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
@@ -387,7 +394,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       // =============================== MMA issuers: one for each row tile ===============================
       const int sub = NSUB == 2 && warp == P::kAux + 3 ? 1 : 0;
       const bool el = elect_one();
-      // (e4m3 has the code of float16 in the descriptor of kind::f8f6f4)
+      // (kind::f8f6f4: e4m3 has the code of float16 in the descriptor, e5m2 that of bfloat16)
       constexpr uint32_t kIdescS = idesc_16<TP>(128, TK, 0), kIdescO = idesc_16<TP>(128, DP, 1);
       const uint64_t qd = smem_desc(sbase + P::kOffQ + sub * P::kQSub, 16, 1024, kLayoutSw128);
       const uint32_t s_at = tmem + P::kColS + 2 * TK * sub, o_at = tmem + P::kColO + sub * DP;
@@ -428,7 +435,8 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
               for (int kk = 0; kk < kTerms * DP / 32; ++kk) {
                 const int term = kk / (DP / 32), in = kk % (DP / 32) * 32;
-                mma8_ss(s_at + TK * buf, qd + (uint64_t)((term * P::kQChunk + in) >> 4), kd + (uint64_t)(in >> 4), kIdescS, kk ? 1u : 0u);
+                mma8_ss(s_at + TK * buf, qd + (uint64_t)((term * P::kQChunk + in) >> 4), kd + (uint64_t)(in >> 4),
+                        kIdescS | (term ? 1u << 7 : 0u), kk ? 1u : 0u);
               }
             } else {
 #pragma unroll
@@ -610,13 +618,9 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               y = make_float2(y.x * f, y.y * f);
 #pragma unroll
               for (int term = 0; term < kTerms; ++term) {
-                const uint32_t lo = e4m3_pair(x), hi = e4m3_pair(y);
+                const uint32_t lo = term == 0 ? take_term<true>(x) : take_term<false>(x);
+                const uint32_t hi = term == 0 ? take_term<true>(y) : take_term<false>(y);
                 codes[term][k / 2] = lo | (hi << 16);
-                if (term < kTerms - 1) {  // what the rounding left: exact
-                  const float2 a2 = e4m3_floats(lo), b2 = e4m3_floats(hi);
-                  x = make_float2(x.x - a2.x, x.y - a2.y);
-                  y = make_float2(y.x - b2.x, y.y - b2.y);
-                }
               }
             }
 #pragma unroll

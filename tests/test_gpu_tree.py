@@ -457,9 +457,10 @@ def test_many_rows_are_merged_together(pkg, Hq, Hkv, dtype, cache):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("rows", [3, 40])
 def test_query_rows_of_a_wide_range_over_e4m3(pkg, dtype, rows):
-    """Q meets an e4m3 cache as two (bfloat16) or three (float16) e4m3 numbers an element, the row's largest between 2^7 and 2^8 and
-    the smallest step 2^-9: what falls below half of that, at most 2^-17 of the row's largest, is lost. A score is off by
-    dq = 2^-17 max|q| sum|k| / sqrt(d) then, a probability by 2 dq, O by 4 dq max|v|. Rows that are not finite are NaN."""
+    """Q meets an e4m3 cache as an e4m3 number and one (bfloat16) or two (float16) e5m2 numbers an element, the row's largest between
+    2^7 and 2^8. Elements from 2^-6 on are held exactly; of smaller ones e4m3 leaves at most 2^-10, and e5m2 (a half step of 2^-3
+    below the power of two) 2^-14 of that: 2^-21 of the row's largest. A score is off by dq = 2^-21 max|q| sum|k| / sqrt(d) then, a
+    probability by 2 dq, O by 4 dq max|v|. Rows that are not finite are NaN."""
     c, Q, cu, mask = problem(dtype, "e4m3", [700], [rows], 8, 2, 128, 16, seed=rows)
     g = torch.Generator().manual_seed(1)
     low = -12 if dtype == "f16" else -24
@@ -467,7 +468,7 @@ def test_query_rows_of_a_wide_range_over_e4m3(pkg, dtype, rows):
     want, bound, written = tree_reference(c, Q, cu, mask)
     k = np.abs(c.dense("K", 0, range(700 + rows))[0]).sum(-1).max()
     v = np.abs(c.dense("V", 0, range(700 + rows))[0]).max()
-    dq = 2.0 ** -17 * np.abs(Q.double().numpy()).max(-1) * k / np.sqrt(128)
+    dq = 2.0 ** -21 * np.abs(Q.double().numpy()).max(-1) * k / np.sqrt(128)
     bound = (bound[0] + dq, bound[1] + 2 * dq * want[1], bound[2] + 4 * (dq * v)[..., None])
     pkg.capi.set_path(pkg.capi.PATH_TILED)
     try:
