@@ -16,13 +16,14 @@
 //   With two row tiles: warps 0-7 softmax, 8-11 the roles of 4-7 (11 the second tile's MMA issuer), 12-19 the conversion.
 // A unit of at most 64 (32) rows has them two (four) times in Q: each copy takes half (a quarter) of every tile's columns, so that all
 // four softmax warps work, and the copies are added up at the end of the piece.
-// An int8 tile meets the tensor cores as float16 numbers that equal its codes, as V of e4m3 does. K of e4m3 meets them as it lies, in the
-// products of 8-bit numbers, and Q as terms of 8 bits, each the rounding of what the terms before left, the first e4m3, the others e5m2. A
-// row is first multiplied by a power of two that brings its largest element to [2^7, 2^8): two terms are a bfloat16 element then, and
-// three a float16 element, exactly, down to 2^-13 of the largest (2^-6, where e4m3's subnormal numbers begin), and smaller ones are held to
-// 2^-21 or 2^-24 of it. (e4m3 alone, which ends at 2^-9, showed in l: 9e-7 of it, float32 sums 4e-7.) Without K's conversion, which
-// passes the tile through shared memory twice: 437 -> 370 us, e4m3 call below. bfloat16 Q over int8 becomes
-// float16 times such a power: none of its 8 bits is lost above 2^-29 of the row's largest element.
+// An 8-bit tile meets the tensor cores as float16 numbers that equal its codes (11 bits hold e4m3 and int8), except K of e4m3 under
+// bfloat16 Q: that meets them as it lies, in the products of 8-bit numbers, and Q as two terms, each the rounding of what is left, the
+// first e4m3, the second e5m2. A row is first multiplied by a power of two that brings its largest element to [2^7, 2^8): the terms are
+// an element exactly then, down to 2^-13 of the largest (2^-6, where e4m3's subnormal numbers begin), and smaller ones are held to 2^-21
+// of it. (e4m3 alone, which ends at 2^-9, showed in l: 9e-7 of it, float32 sums 4e-7.) Without K's conversion, which passes the tile
+// through shared memory twice: 437 -> 370 us, e4m3 call below. float16 elements take three terms, and their products cost more than the
+// conversion: 491 us against 461. bfloat16 Q over int8 becomes float16 times such a power: none of its 8 bits is lost above 2^-29 of the
+// row's largest element.
 // The rows' scales stay in fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the
 // largest of them in.
 // P is rounded to 16 bits. Where that alone would be as large as the rounding of the result (all but 8-bit caches under bfloat16 Q),
@@ -48,8 +49,8 @@ using namespace tile;
 // alone: K and V are fetched and converted once for both.
 template <int DP, class T, class TC, int NSUB>
 struct PlanTree {
-  static constexpr bool kQuant = sizeof(TC) == 1, kRawK = std::is_same<TC, e4m3>::value, kConvertK = kQuant && !kRawK;
-  static constexpr int kTerms = std::is_same<T, __half>::value ? 3 : 2;  // 8-bit numbers of an element of Q (kRawK)
+  static constexpr bool kQuant = sizeof(TC) == 1, kRawK = std::is_same<TC, e4m3>::value && std::is_same<T, __nv_bfloat16>::value, kConvertK = kQuant && !kRawK;
+  static constexpr int kTerms = 2;  // 8-bit numbers of an element of Q (kRawK)
   static constexpr int kSoftmaxWarps = 4 * NSUB, kAux = 4 * NSUB /* first of four warps */, kConvertFrom = kAux + 4;
   static constexpr int kConvert = kQuant ? 128 * NSUB : 0, kThreads = 128 * NSUB + 128 + kConvert, kCtasPerSm = 3 - NSUB;
   static constexpr int kRegsLaunch = NSUB == 1 ? (kQuant ? 80 : 128) : (kQuant ? 96 : 168);
@@ -58,13 +59,13 @@ struct PlanTree {
   static constexpr int kRegsNeeded = kRegsSoftmax * 128 * NSUB + kRegsAux * (kThreads - 128 * NSUB);
   static_assert(kRegsNeeded <= kRegsLaunch * kThreads, "setmaxnreg budgets exceed the launch pool");
   static constexpr int TK = 64, kRows = 128 * NSUB, kChunks = DP / 64;
-  // (two row tiles and e4m3: room for three terms with either type, 160 us against 170 with the stages right behind two)
+  // (two row tiles and kRawK: a term's room is left free, 160 us against 170 with the stages right behind the terms)
   static constexpr int kQChunk = 128 * 128, kKVChunk = TK * 128;
-  static constexpr int kQSub = (!kRawK ? kChunks : NSUB == 2 ? 3 : kTerms) * kQChunk, kQBytes = NSUB * kQSub;
+  static constexpr int kQSub = (!kRawK ? kChunks : NSUB == 2 ? kTerms + 1 : kTerms) * kQChunk, kQBytes = NSUB * kQSub;
   static constexpr int kTile = kChunks * kKVChunk;               // a 16-bit tile of K or V
   static constexpr int kStage = kQuant ? TK * DP : kTile;        // a tile as it is fetched
   static constexpr int kStageK = kRawK ? TK * 128 : kStage;      // K's, where it meets the tensor cores so: in their swizzle
-  static constexpr int NS = (DP == 64 || NSUB == 2) ? 4 : (kRawK && kTerms == 2) ? 3 : 2;  // stages of K and of V: what memory allows
+  static constexpr int NS = (DP == 64 || NSUB == 2) ? 4 : kRawK ? 3 : 2;  // stages of K and of V: what memory allows
   static constexpr int NC = kQuant ? NSUB : 1;                   // converted tiles of K and of V
   static constexpr int kRing = 8;                                // tiles whose masks and scales are kept
   static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStageK, kOffCK = kOffV + NS * kStage;

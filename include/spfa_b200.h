@@ -433,9 +433,8 @@ int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t wid
  *   - probabilities enter the product with V as 16-bit numbers, float16 over an 8-bit cache, else Q's type: two, the rounding and
  *     what it left, where a sequence has at most 128 rows for a key head (tokens x query heads), except over an 8-bit cache under
  *     bfloat16 Q; else one;
- *   - over an e4m3 cache, Q's elements keep their value down to 2^-13 of the largest in their row, and smaller ones are held to
- *     2^-21 of it; a row of Q that is not finite gives NaN;
- *   - over an int8 cache, bfloat16 elements of Q keep theirs down to 2^-29 of the largest in their row;
+ *   - over an e4m3 cache, bfloat16 elements of Q keep their value down to 2^-13 of the largest in their row, and smaller ones are
+ *     held to 2^-21 of it; a row that is not finite gives NaN. Over an int8 cache they keep it down to 2^-29;
  *   - scales of an 8-bit cache are not negative and finite, at most 2^96 of K and 2^100 of V, or NaN: a NaN scale of K or V makes
  *     the rows that see it NaN. V below 2^-71 throughout a sequence loses bits, down to zeros.
  * Everything else is computed in float32.

@@ -457,8 +457,8 @@ def test_many_rows_are_merged_together(pkg, Hq, Hkv, dtype, cache):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("rows", [3, 40])
 def test_query_rows_of_a_wide_range_over_e4m3(pkg, dtype, rows):
-    """Q meets an e4m3 cache as an e4m3 number and one (bfloat16) or two (float16) e5m2 numbers an element, the row's largest between
-    2^7 and 2^8. Elements from 2^-6 on are held exactly; of smaller ones e4m3 leaves at most 2^-10, and e5m2 (a half step of 2^-3
+    """bfloat16 Q meets an e4m3 cache as an e4m3 and an e5m2 number an element, the row's largest between 2^7 and 2^8 (float16 Q meets
+    it as it is, well within these bounds). Elements from 2^-6 on are held exactly; of smaller ones e4m3 leaves at most 2^-10, and e5m2 (a half step of 2^-3
     below the power of two) 2^-14 of that: 2^-21 of the row's largest. A score is off by dq = 2^-21 max|q| sum|k| / sqrt(d) then, a
     probability by 2 dq, O by 4 dq max|v|. Rows that are not finite are NaN."""
     c, Q, cu, mask = problem(dtype, "e4m3", [700], [rows], 8, 2, 128, 16, seed=rows)
