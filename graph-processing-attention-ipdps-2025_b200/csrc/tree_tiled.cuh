@@ -71,7 +71,7 @@ struct PlanTree {
   static constexpr int kOffQ = 0, kOffK = kQBytes, kOffV = kOffK + NS * kStageK, kOffCK = kOffV + NS * kStage;
   static constexpr int kOffCV = kOffCK + (kConvertK ? NC * kTile : 0), kOffScale = kOffCV + (kQuant ? NC * kTile : 0);
   static constexpr int kOffRow = kOffScale + (kQuant ? kRing * 2 * TK * 4 : 0), kOffMask = kOffRow + 128 * 8;
-  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 4 * NS + 4 * NC + 7 * NSUB;
+  static constexpr int kOffBar = kOffMask + kRing * 8, kNumBars = 4 * NS + 4 * NC + 7 * NSUB + 1;
   static constexpr int kOffCut = kOffBar + kNumBars * 8, kOffMisc = kOffCut + (int)sizeof(Cut);
   static constexpr int kDynSmem = kOffMisc + 16 + 1024;
   static_assert(kCtasPerSm * (kDynSmem + 1024) <= 228 * 1024, "shared memory of an SM");
@@ -219,7 +219,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + P::kOffBar + 8u * i; };
   constexpr int B_KFULL = 0, B_KEMPTY = NS, B_VFULL = 2 * NS, B_VEMPTY = 3 * NS, B_CK = 4 * NS /* full [NC], empty [NC] */, B_CV = B_CK + 2 * NC, B_SREADY = B_CK + 4 * NC,
-                B_PREADY = B_SREADY + 2 * NSUB, B_OREADY = B_SREADY + 4 * NSUB /* [sub][buffer] */, B_QFULL = B_SREADY + 6 * NSUB;
+                B_PREADY = B_SREADY + 2 * NSUB, B_OREADY = B_SREADY + 4 * NSUB /* [sub][buffer] */, B_QFULL = B_SREADY + 6 * NSUB, B_GROUP = B_QFULL + NSUB;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::kOffMisc + 4);
   Cut* cut = reinterpret_cast<Cut*>(smem + P::kOffCut);
   uint64_t* ring_mask = reinterpret_cast<uint64_t*>(smem + P::kOffMask);
@@ -248,6 +248,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       mbar_init(bar(B_OREADY + x), 1);
     }
     for (int x = 0; x < NSUB; ++x) mbar_init(bar(B_QFULL + x), 4);
+    mbar_init(bar(B_GROUP), 4);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -563,7 +564,14 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16;
     const uint32_t tO = tmem + lane_base + P::kColO + sub * DP, tS0 = tmem + lane_base + P::kColS + 2 * TK * sub;
     const int b_sready = B_SREADY + 2 * sub, b_pready = B_PREADY + 2 * sub, b_oready = B_OREADY + 2 * sub;
-    auto group_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };  // of units with copies: one sub-tile
+    // The four warps of a unit with copies (one row tile). A barrier that is waited for with a limit, like all others: a warp that gave
+    // up does not come.
+    uint32_t meetings = 0;
+    auto group_sync = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_GROUP));
+      return warp_wait(bar(B_GROUP), meetings++ & 1, abort_flag, err, 313);
+    };
     uint32_t jj = 0, ring = 0;  // tiles of this row tile, and of the CTA
     bool ok = true;
 
@@ -795,7 +803,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       float m = (l_run != l_run && m_true < __int_as_float(0x7f800000)) ? l_run : m_true, l = l_run * rel;
       if constexpr (kCopies > 1) {
         row_ml[tid] = make_float2(m, l);
-        group_sync();
+        if (!group_sync()) return false;
         float top = neg_inf();
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) top = max_nan(top, row_ml[c * kBlock + row].x);
@@ -854,7 +862,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
           for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(smem + P::kOffQ + part * P::kQChunk + P::unit(tid, e / 4)) = four(e);
           if (part < kAtOnce - 1) continue;
-          group_sync();
+          if (!group_sync()) return false;
           for (int x = tid; x < rows * 8 * kAtOnce; x += 128) {
             const int r = x / (8 * kAtOnce), u = x % (8 * kAtOnce), col = (c - part) * 32 + u * 4;
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -865,7 +873,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             }
             if (col < a.d_pad) *reinterpret_cast<float4*>(a.O + (out + r) * a.d_pad + col) = y;
           }
-          group_sync();
+          if (!group_sync()) return false;
         }
       }
       tc_fence_before();
