@@ -113,12 +113,16 @@ int launch_any(const Call& a, const MergeArgs& g, bool vec, cudaStream_t st) {
   return rc != SPFA_OK ? rc : launch_merge_any<TQ, TC>(a, g, vec, st);
 }
 
-// What the copy engine can address: 16-byte rows and strides below 2^40 bytes, boxes that do not cut a page into unaligned pieces.
+// What the copy engine can address: 16-byte rows and strides below 2^40 bytes, boxes that do not cut a page into unaligned pieces. A
+// dimension whose elements share their memory (a tensor expanded over heads: stride 0) is left to the kernels that compute addresses.
 inline bool tiled_shape(const spfa_kv_cache* c) {
   const int size = dtype_bytes(c->dtype);
   if (c->d > 128 || c->n_pages < 1 || !cache_rows_align(c, 16 / size) || (c->page_size % 8 && c->page_size < kTiledKeys)) return false;
-  for (int i = 0; i < 3; ++i)
+  const int64_t count[3] = {c->n_pages, c->page_size, c->n_heads};
+  for (int i = 0; i < 3; ++i) {
     if (c->K_stride[i] * size >= (1LL << 40) || c->V_stride[i] * size >= (1LL << 40)) return false;
+    if (count[i] > 1 && (c->K_stride[i] == 0 || c->V_stride[i] == 0)) return false;
+  }
   return true;
 }
 
@@ -132,7 +136,7 @@ bool make_page_map(CUtensorMap* tm, const spfa_kv_cache* c, void* base, const in
   const cuuint64_t dims[4] = {(cuuint64_t)c->d, (cuuint64_t)c->page_size, (cuuint64_t)c->n_heads, (cuuint64_t)c->n_pages};
   cuuint64_t strides[3] = {(cuuint64_t)stride[1] * sizeof(T), (cuuint64_t)stride[2] * sizeof(T), (cuuint64_t)stride[0] * sizeof(T)};
   for (int i = 0; i < 3; ++i)
-    if (strides[i] == 0) strides[i] = 16;  // of a dimension of one element
+    if (strides[i] == 0) strides[i] = 16;  // of a dimension of one element: tiled_shape lets no other pass
   const cuuint32_t box[4] = {kByte ? (cuuint32_t)bytes : 64u, (cuuint32_t)(c->page_size < kTiledKeys ? c->page_size : kTiledKeys), 1u, 1u};
   const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUtensorMapDataType type = kByte ? CU_TENSOR_MAP_DATA_TYPE_UINT8

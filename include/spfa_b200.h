@@ -428,8 +428,9 @@ int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t wid
  *
  * dtype: type of Q and O (equal to the cache's where that holds its values as they are). float32 calls compute in float32, and so
  * do calls of a few rows over short page lists (one launch). Other 16-bit calls run the committed positions on the tensor cores
- * where d is at most 128, rows are 16-byte aligned (d a multiple of 8, of an 8-bit cache 16) and pages hold a multiple of 8
- * positions or at least 64; with SPFA_PATH_TILED they do or return SPFA_ERR_BAD_ARG, with SPFA_PATH_GATHER they do not. There
+ * where d is at most 128, rows are 16-byte aligned (d a multiple of 8, of an 8-bit cache 16), pages hold a multiple of 8
+ * positions or at least 64, and no stride of K or V is 0 (a tensor expanded over heads) unless its dimension has one element;
+ * with SPFA_PATH_TILED they do or return SPFA_ERR_BAD_ARG, with SPFA_PATH_GATHER they do not. There
  *   - probabilities enter the product with V as 16-bit numbers, float16 over an 8-bit cache, else Q's type: two, the rounding and
  *     what it left, where a sequence has at most 128 rows for a key head (tokens x query heads), except over an 8-bit cache under
  *     bfloat16 Q; else one;
