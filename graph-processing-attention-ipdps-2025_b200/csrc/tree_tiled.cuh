@@ -186,9 +186,10 @@ template <> struct Widen<int8_t> {
   }
 };
 
-// p V_j for an infinite V_j is that infinity, but the products of p's two terms need not add up to it: a term that is zero or negative
-// makes NaN. Where a piece's accumulator is not finite, V itself tells what it has to hold: +inf, -inf, or NaN where both or a NaN are
-// among the keys [p, p_end) that all rows of the piece see. Column `col` of one lane; returned: -1, 1, 2 (NaN) or 0 (all finite).
+// p V_j for an infinite V_j is that infinity, but its products with what stands for p here need not add up to it: a term that is zero or
+// negative makes NaN, and so do the zeros of a copied unit and a p that 16 bits round to zero. Where a piece's accumulator is not finite,
+// V itself tells what it has to hold: +inf, -inf, or NaN where both or a NaN are among the keys [p, p_end) that all rows of the piece
+// see. Column `col` of one lane; returned: -1, 1, 2 (NaN) or 0 (all finite).
 template <class T>
 __device__ __noinline__ int infinity_of(const Call& a, int32_t b, int32_t h, int32_t p, int32_t p_end, int col) {
   const float inf = __int_as_float(0x7f800000);
@@ -834,7 +835,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
 #pragma unroll
         for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * rel);
         if constexpr (!kQuant) {
-          if (split && __any_sync(kFullMask, mine && ((zero[0] | zero[1]) & 0x7fffffff7fffffffull) != 0ull)) {
+          if (__any_sync(kFullMask, mine && ((zero[0] | zero[1]) & 0x7fffffff7fffffffull) != 0ull)) {
             int32_t first, last, slot, end_slot;
             keys_of(w.t0, first, slot);
             const int left = keys_of(w.t0 + w.n - 1, last, end_slot);
