@@ -592,13 +592,17 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P::kRegsSoftmax));
     // =============================== softmax: one thread owns one query row ===============================
-    // P = 2^(s - shift). A row's shift is the maximum it was last set at, less kLift, plus the exponent of the largest of V's scales
-    // (8-bit caches, from 2^-80 on): it is set anew only when that outgrows it by kSlack. A float16 probability times its scale is
-    // below 2^(kLift + kSlack + 1) = 2^15 then, keeps 11 bits down to 2^-22 of its reference and steps of 2^-32 below, so that a
-    // million small ones lose less than 2^-13 of V's magnitude. Each new shift holds a warp up for some 2000 cycles, and the product
-    // with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
+    // P = 2^(s - shift). A row's shift is the maximum it was last set at, less kLift: of s, or over an 8-bit cache of s plus the exponent
+    // of V's scale (from 2^-80 on), as what is rounded to 16 bits is their product. It is set anew only when that maximum outgrows it
+    // by kSlack. Where a tile's scales lie within 2^kNear, as rows of one head do, the largest of them stands for all: a maximum of s
+    // and one exponent. A tile with others takes the maximum over s and its own key's exponent: a large V that a row gives no weight
+    // does not count. (64 tokens of 8 heads over 16384 int8 keys 168 us, 252 where every tile is of the second kind; 32 sequences of up to
+    // 65536 e4m3 keys 724 and 839.) A float16 probability times its scale is below 2^(kLift + kSlack + 1) = 2^15 then, the row's largest is at 2^4 at
+    // least (native caches 2^8), and the others keep 11 bits down to 2^-18 of it and steps of 2^-28 below. Each new shift holds a warp
+    // up for some 2000 cycles, and the product with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
     constexpr bool kHalfP = std::is_same<TP, __half>::value;
     constexpr float kSlack = kHalfP ? 6.f : 8.f, kLift = kHalfP ? 8.f : 0.f;
+    constexpr int kNear = 4;
     const uint64_t minus1 = pack2(-1.f, -1.f);
     constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included
     const int sub = warp / 4, tid = threadIdx.x % 128;
@@ -714,7 +718,6 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
       }
       const bool split = kMaySplit && w.tokens * a.group <= 128;
       float m_true = neg_inf(), shift = neg_inf();
-      float v_ref = -80.f;  // exponent of the largest of V's scales so far
       uint64_t l2[2] = {0ull, 0ull};
       for (int32_t t = 0; t < w.n; ++t, ++jj, ++ring) {
         const uint32_t tS = tS0 + TK * (jj & 1);
@@ -730,11 +733,15 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + ring % P::kRing);
         [[maybe_unused]] const float* scales = ring_scale + (ring % P::kRing) * 2 * TK + col0;
         [[maybe_unused]] const ulonglong2 *ks = reinterpret_cast<const ulonglong2*>(scales), *vs = reinterpret_cast<const ulonglong2*>(scales + TK);
+        [[maybe_unused]] float v_top = 0.f;
+        [[maybe_unused]] bool far = false;
         if constexpr (kQuant) {
           const volatile uint32_t* all = reinterpret_cast<const volatile uint32_t*>(scales + TK - col0);
-          const uint32_t x = all[lane] & 0x7fffffffu, y = all[lane + 32] & 0x7fffffffu;
-          const int top = (int)(__reduce_max_sync(kFullMask, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u)) >> 23) - 127;
-          v_ref = fmaxf(v_ref, (float)min(100, top));
+          // a zero (also: no key) is the last of all numbers less one; NaN the first, but then every row of the unit becomes NaN
+          const uint32_t x = (all[lane] & 0x7fffffffu) - 1u, y = (all[lane + 32] & 0x7fffffffu) - 1u;
+          const int top = __reduce_max_sync(kFullMask, max((int)x, (int)y)) >> 23, low = (int)(__reduce_min_sync(kFullMask, min(x, y)) >> 23);
+          v_top = (float)(min(max(top, 47), 227) - 127);
+          far = top - low > kNear;
         }
         tc_wait_ld();
         if constexpr (kQuant) {
@@ -762,7 +769,26 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], __uint_as_float(sr[e])), __uint_as_float(sr[e + 1]));
         const float t_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
         m_true = fmaxf(m_true, t_max);
-        const float want = kQuant ? t_max + (v_ref - kLift) : t_max - kLift;
+        float want = kQuant ? t_max + (v_top - kLift) : t_max - kLift;
+        if constexpr (kQuant) {
+          if (far) {  // the whole warp; S is read again, 16 columns at a time: unrolled over all, the code would slow the other tiles
+            float best = neg_inf();
+#pragma unroll 1
+            for (int c = 0; c < kCols; c += 16) {
+              uint32_t s16[16];
+              tmem_ld16(tS + col0 + c, s16);
+              tc_wait_ld();
+              const uint32_t here = (uint32_t)(mask >> (col0 + c));
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t biased = min(max(__float_as_uint(scales[TK + c + e]) >> 23 & 0xffu, 47u), 227u);
+                const float s = __uint_as_float(s16[e]) * scales[c + e] * sc + (__uint_as_float(0x4b000000u | biased) - 8388735.f);
+                if ((here >> e) & 1u) best = fmaxf(best, s);
+              }
+            }
+            want = best - kLift;
+          }
+        }
         const bool move = want > shift + kSlack;
         if (__any_sync(kFullMask, move)) {
           const float new_shift = move ? want : shift;

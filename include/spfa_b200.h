@@ -436,8 +436,12 @@ int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t wid
  *     bfloat16 Q; else one;
  *   - over an e4m3 cache, bfloat16 elements of Q keep their value down to 2^-13 of the largest in their row, and smaller ones are
  *     held to 2^-21 of it; a row that is not finite gives NaN. Over an int8 cache they keep it down to 2^-29;
+ *   - over an 8-bit cache that number holds a probability times the scale of V: to 11 bits (22 where there are two), or to 2^-29 of the
+ *     row's largest such product, whichever is more: keys whose product lies below that add less than their part, or nothing. Keys
+ *     that a row gives no weight do not change this, whatever their V is;
  *   - scales of an 8-bit cache are not negative and finite, at most 2^96 of K and 2^100 of V, or NaN: a NaN scale of K or V makes
- *     the rows that see it NaN. V below 2^-71 throughout a sequence loses bits, down to zeros.
+ *     the rows that see it NaN. Rows above that (append holds values up to the largest of float32: scales up to 2^121) give infinities
+ *     or NaN. V below 2^-71 throughout a sequence loses bits, down to zeros.
  * Everything else is computed in float32.
  * The workspace needs spfa_tree_workspace_bytes of the same cache, n_rows and n_q_heads. */
 size_t spfa_tree_workspace_bytes(const spfa_kv_cache* cache, int dtype, int64_t n_rows, int64_t n_q_heads);
