@@ -792,10 +792,16 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const bool move = want > shift + kSlack;
         if (__any_sync(kFullMask, move)) {
           const float new_shift = move ? want : shift;
-          const float f = move ? ((shift == neg_inf()) ? 0.f : fast_exp2(shift - new_shift)) : 1.0f;
+          // Scales lie up to 2^180 apart, and so do shifts, whatever the scores are: what a factor of 2^-180 leaves of l may still be most
+          // of it. So the factor's root, twice.
+          const float f = move ? ((shift == neg_inf()) ? 0.f : fast_exp2(kQuant ? 0.5f * (shift - new_shift) : shift - new_shift)) : 1.0f;
           const uint64_t f2 = pack2(f, f);
-          l2[0] = fma2(l2[0], f2, 0ull);
-          l2[1] = fma2(l2[1], f2, 0ull);
+#pragma unroll
+          for (int i = 0; i < (kQuant ? 2 : 1); ++i) {
+            l2[0] = fma2(l2[0], f2, 0ull);
+            l2[1] = fma2(l2[1], f2, 0ull);
+          }
+          const float f_O = kQuant ? f * f : f;
           if (t > 0) {  // O of this row up to the previous tile is final once that tile's barrier has completed
             if (!warp_wait(bar(b_oready + ((jj - 1) & 1)), ((jj - 1) >> 1) & 1, abort_flag, err, 312)) return false;
             tc_fence_after();
@@ -805,7 +811,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
               tmem_ld32(tO + c * 32, ob);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * f);
+              for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(__uint_as_float(ob[e]) * f_O);
               tmem_st32(tO + c * 32, ob);
             }
           }

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import cache_ref
 from test_gpu_tree import both_paths, problem
 from tree_tight import check_path
 
@@ -61,7 +62,7 @@ def test_a_large_row_that_nobody_attends_to(pkg, rows, dtype, cache):
 
 @pytest.mark.parametrize("dtype,cache", EIGHT)
 @pytest.mark.parametrize("rows", [3, 20, 70])
-@pytest.mark.parametrize("spread", [1, 3, 8])
+@pytest.mark.parametrize("spread", [2, 8])
 def test_scales_of_a_wide_range(pkg, spread, rows, dtype, cache):
     """Every V row times a power of two between 2^-spread and 2^spread."""
     c, _, cu, mask = long_problem(dtype, cache, rows, seed=spread)
@@ -70,3 +71,36 @@ def test_scales_of_a_wide_range(pkg, spread, rows, dtype, cache):
     for b, n in enumerate(LENS):
         set_rows(c, "V", b, range(n + rows), 2.0 ** rng.integers(-spread, spread + 1, n + rows))
     assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "int8"), ("bf16", "e4m3"), ("bf16", "int8")])
+@pytest.mark.parametrize("rows", [3, 20, 70])
+@pytest.mark.parametrize("low,high", [(-64, 0), (-64, 90), (0, -64), (90, -64), (90, 90)])
+def test_scales_from_end_to_end_of_what_is_held(pkg, low, high, rows, dtype, cache):
+    """Every other 128 keys lie far from the rest, and attention is on both, or twelve apart: l counts every key, whatever its V."""
+    for lift in (0.0, 12.0, -12.0) if low * high < 0 else (0.0,):
+        c, Q, cu, mask = long_problem(dtype, cache, rows, seed=5)
+        for b, n in enumerate(LENS):
+            far = [p for p in range(n + rows) if p // 128 % 2 == 0]
+            set_rows(c, "V", b, far, 2.0 ** low)
+            set_rows(c, "V", b, [p for p in range(n + rows) if p // 128 % 2], 2.0 ** high)
+            if lift:
+                set_keys(c, b, far, lift)
+        assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2
+
+
+@pytest.mark.parametrize("dtype,cache", EIGHT)
+@pytest.mark.parametrize("rows", [3, 70])
+def test_rows_of_zeros_beside_large_ones(pkg, rows, dtype, cache):
+    """A V row of zeros has the smallest scale there is (int8: zero), and its key counts in l all the same."""
+    c, Q, cu, mask = long_problem(dtype, cache, rows, seed=4)
+    _, scale = cache_ref.quantise(np.zeros((16, 64)), cache)
+    for b, n in enumerate(LENS):
+        at = places(c, b, list(range(70)) + [n // 2, n - 1] + list(range(320, 320 + 64 * (b % 3))))
+        c.V.view(torch.uint8)[at] = 0
+        c.V_scale[at] = torch.from_numpy(scale).to(c.V_scale)
+    assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2
+    if dtype != "f16":
+        for b, n in enumerate(LENS):
+            set_rows(c, "V", b, range(100, n + rows), 2.0 ** 50)
+        assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2

@@ -46,6 +46,8 @@ def tree_tight(c, Q, cu, mask, tag):
         w = min(T, mask.shape[1])
         seen[:, n:n + w] = mask[n0:n1, :w].numpy()
         seen &= ok[None]
+        if vs is not None:
+            v_scale = np.array([vs[c.place(b, i)] if ok[i] else np.zeros(c.heads) for i in range(n)]).reshape(n, c.heads)
         for h in range(Hq):
             x, kk, vv = q[n0:n1, h], k[:, h // g], v[:, h // g]
             some = seen.any(-1)
@@ -66,9 +68,7 @@ def tree_tight(c, Q, cu, mask, tag):
             size = p @ np.abs(vv) / ll[:, None]
             e = 2 * rel[:, None] * size + one * (p[:, :n] @ np.abs(vv[:n])) / ll[:, None]
             if step and n:
-                scale = np.ones(n)
-                if vs is not None:
-                    scale = np.array([vs[c.place(b, i)][h // g] if ok[i] else 0.0 for i in range(n)])
+                scale = np.ones(n) if vs is None else v_scale[:, h // g]
                 codes = np.abs(np.divide(vv[:n], scale[:, None], out=np.zeros_like(vv[:n]), where=scale[:, None] != 0))
                 e = e + step * (p[:, :n] * scale).max(-1, keepdims=True) * codes.sum(0)[None] / ll[:, None]
             o = p @ vv / ll[:, None]
