@@ -1,0 +1,61 @@
+"""GPU: the attention of drafted trees within bounds that know which kernel ran (tree_tight): probabilities in two terms where they are
+promised, one where not, none rounded in the kernels without tensor cores. Pieces of several tiles, and more sequences than threads."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_tree import DT, SHAPES, TYPES, both_paths, problem, run
+from tree_tight import check_path, few_keys
+
+pytestmark = pytest.mark.gpu
+
+
+def check_all(pkg, c, Q, cu, mask):
+    known, tags = {}, []
+    for tag, got in both_paths(pkg, c, Q, cu, mask):
+        check_path(pkg, c, Q, cu, mask, tag, got, known)
+        tags.append(tag)
+    return tags
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("rows", [[5, 3], [40, 20]])
+def test_probabilities_in_the_promised_bits(pkg, rows, dtype, cache):
+    c, Q, cu, mask = few_keys(DT[dtype], cache, rows)
+    assert ("tiled" in check_all(pkg, c, Q, cu, mask)) == (dtype != "f32")
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_shapes(pkg, shape, dtype, cache):
+    lens, rows, Hq, Hkv, d, page, layout = shape
+    check_all(pkg, *problem(dtype, cache, lens, rows, Hq, Hkv, d, page, layout, seed=d + page))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("rows,d,page,q_scale", [(3, 128, 16, 1.0), (20, 64, 24, 6.0), (40, 80, 64, 2.0), (70, 64, 100, 4.0)])
+def test_pieces_of_several_tiles(pkg, rows, d, page, q_scale, dtype, cache):
+    """Units of 6, 40, 80 and 140 rows, whose running maximum moves from tile to tile."""
+    c, Q, cu, mask = problem(dtype, cache, [900, 800, 700], [rows] * 3, 32, 16, d, page, "hnd", seed=rows, q_scale=q_scale)
+    check_all(pkg, c, Q, cu, mask)
+
+
+@pytest.mark.parametrize("dtype,cache", [("f32", "native"), ("bf16", "native"), ("f16", "int8"), ("bf16", "e4m3")])
+def test_more_sequences_than_threads(pkg, dtype, cache):
+    """The list of key tiles is cut by a scan over the sequences, a CTA's threads at a time: 700 of them, some without rows or keys."""
+    rng = np.random.default_rng(3)
+    lens, rows = rng.integers(0, 40, 700), rng.integers(0, 4, 700)
+    lens[rng.integers(0, 700, 60)] = 0
+    lens[[255, 256, 257, 383, 384, 385, 639, 640, 641, 699]] = 39
+    rows[[255, 256, 257, 383, 384, 385, 639, 640, 641, 699]] = 2
+    c, Q, cu, mask = problem(dtype, cache, lens.tolist(), rows.tolist(), 2, 1, 16, 8, seed=1)
+    assert ("tiled" in check_all(pkg, c, Q, cu, mask)) == (dtype != "f32")
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_a_call_repeats_itself_bit_for_bit(pkg, dtype, cache):
+    for rows, heads in (([3, 9, 1], 8), ([80, 40, 20], 16), ([1, 0, 2], 2)):
+        c, Q, cu, mask = problem(dtype, cache, [1900, 300, 700], rows, heads, 2, 64, 16, seed=rows[0])
+        first = run(pkg, c, Q, cu, mask)
+        for _ in range(5):
+            assert all(torch.equal(x, y) for x, y in zip(run(pkg, c, Q, cu, mask), first))

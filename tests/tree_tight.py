@@ -3,7 +3,7 @@ bits, on the CPU; used by the tests only. cache_ref.tree_reference has one bound
 import numpy as np
 import torch
 
-from cache_ref import HALF, check_tree
+from cache_ref import HALF, Cache, check_tree
 
 U = 2.0 ** -24
 
@@ -78,6 +78,18 @@ def tree_tight(c, Q, cu, mask, tag):
             em[n0:n1, h], el[n0:n1, h] = ds + 4 * U * np.abs(top), rel * ll
             eO[n0:n1, h] = e + half * (np.abs(o) + e)
     return (m, l, O), (em, el, eO), written
+
+
+def few_keys(dtype, cache, rows, device="cuda"):
+    """(cache, Q, cu_rows, mask) where little but the rounding of probabilities can move a result: nine and five keys of 16 elements, one
+    element of a query that is not zero, and columns of O in which V's signs cancel, so that the result's own rounding is small."""
+    lens = [9, 5]
+    c = Cache(dtype, cache, [n + r for n, r in zip(lens, rows)], 2, 16, 16, "nhd", 3, lens, device=device)
+    g = torch.Generator().manual_seed(4)
+    Q = torch.zeros(sum(rows), 8, 16)
+    Q.scatter_(2, torch.randint(0, 16, (sum(rows), 8, 1), generator=g), torch.randn(sum(rows), 8, 1, generator=g) * 4)
+    mask = torch.rand(sum(rows), max(rows), generator=g) < 0.1
+    return c, Q.to(dtype), [0, rows[0], sum(rows)], mask
 
 
 def check_path(pkg, c, Q, cu, mask, tag, got, known):
