@@ -37,6 +37,22 @@ inline int check_cache(const spfa_kv_cache* c, int dtype) {
   return SPFA_OK;
 }
 
+// Whether every element of something that a call writes has a place of its own, as far as strides of 0 tell.
+inline bool apart(const int64_t* count, const int64_t* stride, int n) {
+  for (int i = 0; i < n; ++i)
+    if (count[i] > 1 && stride[i] == 0) return false;
+  return true;
+}
+// check_cache of a call that writes into the cache.
+inline int check_written_cache(const spfa_kv_cache* c, int dtype) {
+  const int rc = check_cache(c, dtype);
+  if (rc != SPFA_OK) return rc;
+  const int64_t count[3] = {c->n_pages, c->page_size, c->n_heads};
+  if (!apart(count, c->K_stride, 3) || !apart(count, c->V_stride, 3)) return SPFA_ERR_BAD_ARG;
+  if (dtype_bytes(c->dtype) == 1 && (!apart(count, c->K_scale_stride, 3) || !apart(count, c->V_scale_stride, 3))) return SPFA_ERR_BAD_ARG;
+  return SPFA_OK;
+}
+
 inline CacheView cache_view(const spfa_kv_cache* c) {
   CacheView v{};
   v.K.data = static_cast<char*>(c->K);

@@ -63,9 +63,11 @@ int launch_rows(const spfa_kv_cache* c, const cache::RowsView& rows, cudaStream_
 template <bool kAppend>
 int rows_call(const spfa_kv_cache* c, int dtype, void* K, const int64_t* ks, void* V, const int64_t* vs, const int32_t* cu,
               int64_t n_rows, void* stream) {
-  int rc = check_cache(c, dtype);
+  int rc = kAppend ? check_written_cache(c, dtype) : check_cache(c, dtype);
   if (rc == SPFA_OK) rc = check_rows_arg(K, ks, V, vs, cu, n_rows, dtype);
   if (rc != SPFA_OK) return rc;
+  const int64_t count[2] = {n_rows, c->n_heads};
+  if (!kAppend && (!apart(count, ks, 2) || !apart(count, vs, 2))) return SPFA_ERR_BAD_ARG;
   if (n_rows == 0 || c->n_seq == 0 || c->n_pages == 0 || c->table_width == 0) return SPFA_OK;
   cache::RowsView rows{static_cast<char*>(K), static_cast<char*>(V), {ks[0], ks[1]}, {vs[0], vs[1]}, cu, n_rows, 0};
   return with_cache_types(dtype, c->dtype, [&](auto* t, auto* tc) {
@@ -93,7 +95,7 @@ int spfa_cache_read(const spfa_kv_cache* c, int dtype, void* K, const int64_t* K
 }
 
 int spfa_cache_keep(const spfa_kv_cache* c, const int32_t* kept, int64_t width, const int32_t* n_kept, void* stream) {
-  const int rc = check_cache(c, -1);
+  const int rc = check_written_cache(c, -1);
   if (rc != SPFA_OK) return rc;
   if (width < 0 || (width > 0 && !kept) || !n_kept || !aligned4(kept) || !aligned4(n_kept)) return SPFA_ERR_BAD_ARG;
   if (width > kMost32 || c->n_seq * c->n_heads > kMost32) return SPFA_ERR_TOO_LARGE;

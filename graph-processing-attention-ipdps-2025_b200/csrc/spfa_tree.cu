@@ -84,6 +84,8 @@ int spfa_tree_forward(const spfa_kv_cache* c, int dtype, const void* Q, const in
   if (!Q || !Q_stride || !cu_rows || !m || !l || !O || !O_stride || mask_width < 0 || (mask_width > 0 && !tree_mask)) return SPFA_ERR_BAD_ARG;
   if (!aligned_to(Q, size) || !aligned_to(O, size) || !aligned4(cu_rows) || !aligned4(m) || !aligned4(l)) return SPFA_ERR_BAD_ARG;
   if (Q_stride[0] < 0 || Q_stride[1] < 0 || O_stride[0] < 0 || O_stride[1] < 0) return SPFA_ERR_BAD_ARG;
+  const int64_t count[2] = {n_rows, n_q_heads};
+  if (!apart(count, O_stride, 2)) return SPFA_ERR_BAD_ARG;
   const TreeLayout t = tree_layout(c, dtype, n_rows, n_q_heads);
   rc = check_workspace(workspace, workspace_bytes, t.total);
   if (rc != SPFA_OK) return rc;
