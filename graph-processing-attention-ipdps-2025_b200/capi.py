@@ -529,6 +529,7 @@ class KvCache(ctypes.Structure):
                 ("n_pages", ctypes.c_int64), ("page_size", ctypes.c_int64), ("n_heads", ctypes.c_int64),
                 ("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("n_seq", ctypes.c_int64),
                 ("table_width", ctypes.c_int64), ("d", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+    device = None  # of the tensors that kv_cache described
 
 
 ROWS_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -568,7 +569,14 @@ def kv_cache(K_pages, V_pages, page_table, lens, K_scale=None, V_scale=None) -> 
     c.page_table, c.lens = page_table.data_ptr(), lens.data_ptr()
     c.n_seq, c.table_width = page_table.shape
     c.dtype = CACHE_CODE[K_pages.dtype]
+    c.device = dev
     return c
+
+
+def _on_cache(cache, dev):
+    """The rows' device has to be the cache's: a kernel would take the cache's addresses for its own device's."""
+    if cache.device is not None and cache.device != dev:
+        raise SpfaError(-1, f"the cache is on {cache.device}, the call's tensors are on {dev}")
 
 
 def _i32(dev, **ts):
@@ -601,6 +609,7 @@ def _cu(dev, cache, cu_rows):
 def cache_append(cache: KvCache, K, V, cu_rows):
     """Write the rows K, V [n, heads, d] to their positions in the cache, in its type."""
     dev = cu_rows.device
+    _on_cache(cache, dev)
     code = _rows3(dev, cache, cache.n_heads, K, V)
     with torch.cuda.device(dev):
         if K.shape[0] and cache.n_seq:
@@ -611,6 +620,7 @@ def cache_append(cache: KvCache, K, V, cu_rows):
 def cache_read(cache: KvCache, K, V, cu_rows):
     """Fill the rows K, V [n, heads, d] from their positions in the cache."""
     dev = cu_rows.device
+    _on_cache(cache, dev)
     code = _rows3(dev, cache, cache.n_heads, K, V)
     with torch.cuda.device(dev):
         if K.shape[0] and cache.n_seq:
@@ -622,6 +632,7 @@ def cache_read(cache: KvCache, K, V, cu_rows):
 def cache_keep(cache: KvCache, kept, n_kept):
     """Move position lens[b] + kept[b, i] to lens[b] + i for i < n_kept[b]; kept is ascending."""
     dev = kept.device
+    _on_cache(cache, dev)
     _i32(dev, kept=kept, n_kept=n_kept)
     if kept.dim() != 2 or kept.shape[0] != cache.n_seq or tuple(n_kept.shape) != (cache.n_seq,):
         raise SpfaError(-1, "kept [sequences, width] and n_kept [sequences] must have one row per sequence")
@@ -633,6 +644,7 @@ def cache_keep(cache: KvCache, kept, n_kept):
 def tree_forward(cache: KvCache, Q, cu_rows, tree_mask, m, l, O, first=False):
     """Attention of the drafted rows Q [n, query heads, d] over the cache (include/spfa_b200.h: spfa_tree_forward)."""
     dev = cu_rows.device
+    _on_cache(cache, dev)
     n, heads = Q.shape[:2]
     code = _rows3(dev, cache, heads, Q, O)
     if tree_mask.dtype not in (torch.bool, torch.uint8) or tree_mask.dim() != 2 or tree_mask.shape[0] != n \

@@ -395,8 +395,9 @@ int spfa_global_no_local_forward_16(int dtype, const void* Q, const void* K, con
  * position does not exist: a position at or behind table_width * page_size, from 2^31 - 1 on, or in a page whose number is not in
  * [0, n_pages), is neither read nor written, and nobody attends to it. Lengths below 0 count as 0 where keys are counted.
  * Sequences may share pages. A call that writes one position twice (two sequences with that page, or a page listed twice) may leave
- * parts of both rows there, and a code beside the other row's scale: write it once. What a call writes (the cache of append and keep with its scales, the rows of read, O) has a place for
- * every element: a stride of 0 over more than one is SPFA_ERR_BAD_ARG. What is only read may be expanded so. */
+ * parts of both rows there, and a code beside the other row's scale: write it once. What a call writes (the cache of append and
+ * keep with its scales, the rows of read, O) has a place for every element: a stride of 0 over more than one is SPFA_ERR_BAD_ARG.
+ * What is only read may be expanded so. */
 enum { SPFA_DTYPE_E4M3 = 3, SPFA_DTYPE_INT8 = 4 };
 typedef struct spfa_kv_cache {
   void *K, *V;
