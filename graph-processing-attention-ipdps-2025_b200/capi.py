@@ -539,7 +539,7 @@ CACHE_CODE = {**ROWS_CODE, torch.float8_e4m3fn: 3, torch.int8: 4}
 def kv_cache(K_pages, V_pages, page_table, lens, K_scale=None, V_scale=None) -> KvCache:
     """Describe a paged cache: pages [n_pages, page_size, heads, d] (float32, float16, bfloat16, float8_e4m3fn or int8; last
     dimension contiguous), page_table [sequences, pages] and lens [sequences] int32, and for the 8-bit types the scales
-    [n_pages, page_size, heads] float32. The description holds addresses: the tensors have to outlive it."""
+    [n_pages, page_size, heads] float32. The description holds the tensors' addresses, and keeps the tensors for as long as it lives."""
     dev = K_pages.device
     if not K_pages.is_cuda:
         raise SpfaError(-1, "tensors must be CUDA tensors (there is no CPU path)")
@@ -570,6 +570,7 @@ def kv_cache(K_pages, V_pages, page_table, lens, K_scale=None, V_scale=None) -> 
     c.n_seq, c.table_width = page_table.shape
     c.dtype = CACHE_CODE[K_pages.dtype]
     c.device = dev
+    c.tensors = (K_pages, V_pages, page_table, lens, K_scale, V_scale)
     return c
 
 
