@@ -51,7 +51,8 @@ bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t*
 constexpr double kDirectRounds = 1;
 bool direct_call(const tree::Call& a, const spfa_kv_cache* c, bool vec) {
   const int size = dtype_bytes(c->dtype);
-  if (!vec || c->d > 128 || !cache_rows_align(c, 16 / size)) return false;
+  // (a cache without pages has no address that a copy of nothing could name)
+  if (!vec || c->d > 128 || c->n_pages < 1 || !cache_rows_align(c, 16 / size)) return false;
   const double waves = (double)((a.n_rows * c->n_heads * ((a.group + tree::kDirectRows - 1) / tree::kDirectRows) + 147) / 148);
   const int keys = tree::DirectPlan(c->d * size).warps * 32;
   return waves * (double)((a.c.capacity + keys - 1) / keys) <= kDirectRounds;
