@@ -556,17 +556,20 @@ def kv_cache(K_pages, V_pages, page_table, lens, K_scale=None, V_scale=None) -> 
     for t in (V_pages,) + ((K_scale, V_scale) if quantised else ()):
         if t.device != dev:
             raise SpfaError(-1, "the tensors of a cache must be on one device")
+    def at(t):  # an empty tensor has no address, and nothing is read through this one
+        return t.data_ptr() or 4096
+
     c = KvCache()
-    c.K, c.V = K_pages.data_ptr(), V_pages.data_ptr()
+    c.K, c.V = at(K_pages), at(V_pages)
     c.K_stride[:], c.V_stride[:] = K_pages.stride()[:3], V_pages.stride()[:3]
     if quantised:
         for t in (K_scale, V_scale):
             if t.dtype != torch.float32 or t.shape != K_pages.shape[:3]:
                 raise SpfaError(-1, "K_scale and V_scale must be float32 [n_pages, page_size, heads]")
-        c.K_scale, c.V_scale = K_scale.data_ptr(), V_scale.data_ptr()
+        c.K_scale, c.V_scale = at(K_scale), at(V_scale)
         c.K_scale_stride[:], c.V_scale_stride[:] = K_scale.stride(), V_scale.stride()
     c.n_pages, c.page_size, c.n_heads, c.d = K_pages.shape
-    c.page_table, c.lens = page_table.data_ptr(), lens.data_ptr()
+    c.page_table, c.lens = at(page_table), at(lens)
     c.n_seq, c.table_width = page_table.shape
     c.dtype = CACHE_CODE[K_pages.dtype]
     c.device = dev
