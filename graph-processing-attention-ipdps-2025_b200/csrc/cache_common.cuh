@@ -21,6 +21,12 @@ struct e4m3 {
   uint8_t bits;
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // One 32-bit value of an element, and back (rounding to nearest even; e4m3 saturates at 448).
 __device__ __forceinline__ float up1(float x) { return x; }
 __device__ __forceinline__ float up1(__half x) { return __half2float(x); }

@@ -17,12 +17,6 @@ struct RowsView {  // rows of a call: [n_rows, heads, d], d contiguous
   int64_t first;  // of the launch: its group numbers are 32-bit
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 // Where row i of a call lies in the cache; page -1: nowhere.
 struct Place {
   int32_t page, slot;

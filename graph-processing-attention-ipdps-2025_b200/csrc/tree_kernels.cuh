@@ -18,12 +18,6 @@
 namespace spfa {
 namespace tree {
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 struct Call {
   CacheView c;
   const char* Q;
