@@ -59,3 +59,14 @@ def test_a_call_repeats_itself_bit_for_bit(pkg, dtype, cache):
         first = run(pkg, c, Q, cu, mask)
         for _ in range(5):
             assert all(torch.equal(x, y) for x, y in zip(run(pkg, c, Q, cu, mask), first))
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+def test_a_chunk_of_a_prompt(pkg, dtype, cache):
+    """Hundreds of rows that see the committed positions and one another causally, ragged, beside a single token."""
+    rows = [300, 1, 65]
+    c, Q, cu, _ = problem(dtype, cache, [200, 90, 0], rows, 4, 2, 64, 16, seed=2)
+    mask = torch.zeros(sum(rows), max(rows), dtype=torch.bool)
+    for b, T in enumerate(rows):
+        mask[cu[b]:cu[b + 1], :T] = torch.ones(T, T, dtype=torch.bool).tril()
+    check_all(pkg, c, Q, cu, mask)

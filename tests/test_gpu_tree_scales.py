@@ -73,6 +73,18 @@ def test_scales_of_a_wide_range(pkg, spread, rows, dtype, cache):
     assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2
 
 
+@pytest.mark.parametrize("dtype,cache", EIGHT)
+@pytest.mark.parametrize("rows", [3, 20, 70])
+def test_key_scales_of_a_wide_range(pkg, rows, dtype, cache):
+    """Every K row times a power of two between 2^-10 and 2^2: scores from almost nothing to some twenty."""
+    c, _, cu, mask = long_problem(dtype, cache, rows, seed=7)
+    Q = (torch.randn(3 * rows, 32, 64, generator=torch.Generator().manual_seed(1)) * 2).to(c.dtype)
+    rng = np.random.default_rng(rows)
+    for b, n in enumerate(LENS):
+        set_rows(c, "K", b, range(n + rows), 2.0 ** rng.integers(-10, 3, n + rows))
+    assert len(list(check_paths(pkg, c, Q, cu, mask))) >= 2
+
+
 @pytest.mark.parametrize("dtype,cache", [("f32", "int8"), ("bf16", "e4m3"), ("bf16", "int8")])
 @pytest.mark.parametrize("rows", [3, 20, 70])
 @pytest.mark.parametrize("low,high", [(-64, 0), (-64, 90), (0, -64), (90, -64), (90, 90)])
