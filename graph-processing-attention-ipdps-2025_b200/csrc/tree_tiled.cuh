@@ -128,6 +128,12 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void mma8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -394,7 +400,7 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
                   cp_async4(dst + 128 * x, ks[x] + page * a.c.K.s_stride[0] + slot * a.c.K.s_stride[1]);
                   cp_async4(dst + 128 * x + TK * 4, vs[x] + page * a.c.V.s_stride[0] + slot * a.c.V.s_stride[1]);
                 } else {
-                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128 * x), "f"(0.f) : "memory");
+                  asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128 * x), "f"(1.f) : "memory");  // its score is -inf, and stays that
                   asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 128 * x + TK * 4), "f"(0.f) : "memory");
                 }
               }
@@ -594,12 +600,15 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     // =============================== softmax: one thread owns one query row ===============================
     // P = 2^(s - shift). A row's shift is the maximum it was last set at, less kLift: of s, or over an 8-bit cache of s plus the exponent
     // of V's scale (from 2^-80 on), as what is rounded to 16 bits is their product. It is set anew only when that maximum outgrows it
-    // by kSlack. Where a tile's scales lie within 2^kNear, as rows of one head do, the largest of them stands for all: a maximum of s
-    // and one exponent. A tile with others takes the maximum over s and its own key's exponent: a large V that a row gives no weight
-    // does not count. (64 tokens of 8 heads over 16384 int8 keys 168 us, 252 where every tile is of the second kind; 32 sequences of up to
-    // 65536 e4m3 keys 724 and 839.) A float16 probability times its scale is below 2^(kLift + kSlack + 1) = 2^15 then, the row's largest is at 2^4 at
-    // least (native caches 2^8), and the others keep 11 bits down to 2^-18 of it and steps of 2^-28 below. Each new shift holds a warp
-    // up for some 2000 cycles, and the product with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
+    // by kSlack. A maximum of s and the tile's largest exponent bounds it; where that would set it anew and the tile's scales lie more
+    // than 2^kNear apart, the maximum is taken key by key: a large V that a row gives no weight does not count. (64 tokens of 8 heads
+    // over 16384 int8 keys 170 us, 265 where scales from 2^-4 to 2^4 are mixed in every tile; 32 sequences of up to 65536 e4m3 keys 712
+    // and 744.) A float16 probability times its scale is below 2^(kLift + kSlack + 1) = 2^15 then, the row's largest is at 2^4 at least
+    // (native caches 2^8), and the others keep 11 bits down to 2^-18 of it and steps of 2^-28 below. Each new shift holds a warp up for
+    // some 2000 cycles, and the product with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
+    // What few tiles need (keys that do not exist, scales far apart) is written small, in a loop over columns that are read from tensor
+    // memory again: the code of the other tiles, with that of the other roles, just fits the instruction cache. All of it in registers,
+    // calls of 128 rows a unit over 8-bit caches took up to 20 % longer, with four times the cache's misses.
     constexpr bool kHalfP = std::is_same<TP, __half>::value;
     constexpr float kSlack = kHalfP ? 6.f : 8.f, kLift = kHalfP ? 8.f : 0.f;
     constexpr int kNear = 4;
@@ -723,6 +732,21 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
         const uint32_t tS = tS0 + TK * (jj & 1);
         if (!warp_wait(bar(b_sready + (jj & 1)), (jj >> 1) & 1, abort_flag, err, 311)) return false;
         tc_fence_after();
+        const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + ring % P::kRing);
+        if (mask != ~0ull) {  // keys that do not exist
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 16) {
+            uint32_t s16[16];
+            tmem_ld16(tS + col0 + c, s16);
+            tc_wait_ld();
+            const uint32_t here = (uint32_t)(mask >> (col0 + c));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s16[e] = (here >> e) & 1u ? s16[e] : 0xff800000u;
+            tmem_st8(tS + col0 + c, *reinterpret_cast<const uint32_t(*)[8]>(s16));
+            tmem_st8(tS + col0 + c + 8, *reinterpret_cast<const uint32_t(*)[8]>(s16 + 8));
+          }
+          tc_wait_st();
+        }
         uint32_t sr[kCols];
         if constexpr (kCols == 16) tmem_ld16(tS + col0, sr);
         if constexpr (kCols == 32) tmem_ld32(tS + col0, sr);
@@ -730,18 +754,13 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
           tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(sr));
           tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(sr + 32));
         }
-        const uint64_t mask = *reinterpret_cast<volatile uint64_t*>(ring_mask + ring % P::kRing);
         [[maybe_unused]] const float* scales = ring_scale + (ring % P::kRing) * 2 * TK + col0;
         [[maybe_unused]] const ulonglong2 *ks = reinterpret_cast<const ulonglong2*>(scales), *vs = reinterpret_cast<const ulonglong2*>(scales + TK);
-        [[maybe_unused]] float v_top = 0.f;
-        [[maybe_unused]] bool far = false;
+        [[maybe_unused]] int v_top = 0;  // exponent of the largest of V's scales here, with its bias
         if constexpr (kQuant) {
           const volatile uint32_t* all = reinterpret_cast<const volatile uint32_t*>(scales + TK - col0);
-          // a zero (also: no key) is the last of all numbers less one; NaN the first, but then every row of the unit becomes NaN
-          const uint32_t x = (all[lane] & 0x7fffffffu) - 1u, y = (all[lane + 32] & 0x7fffffffu) - 1u;
-          const int top = __reduce_max_sync(kFullMask, max((int)x, (int)y)) >> 23, low = (int)(__reduce_min_sync(kFullMask, min(x, y)) >> 23);
-          v_top = (float)(min(max(top, 47), 227) - 127);
-          far = top - low > kNear;
+          // NaN is the largest, but then every row of the unit becomes NaN
+          v_top = (int)(__reduce_max_sync(kFullMask, max(all[lane] & 0x7fffffffu, all[lane + 32] & 0x7fffffffu)) >> 23);
         }
         tc_wait_ld();
         if constexpr (kQuant) {
@@ -757,40 +776,41 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
             sr[e + 3] = __float_as_uint(x3);
           }
         }
-        if (mask != ~0ull) {
-          const uint64_t here = mask >> col0;
-          const uint32_t lo = (uint32_t)here, hi = (uint32_t)(here >> 32);
-#pragma unroll
-          for (int e = 0; e < kCols; ++e) sr[e] = (((e < 32 ? lo : hi) >> (e & 31)) & 1u) ? sr[e] : 0xff800000u;
-        }
         float mx[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
 #pragma unroll
         for (int e = 0; e < kCols; e += 2)
           mx[(e >> 1) & 3] = fmaxf(fmaxf(mx[(e >> 1) & 3], __uint_as_float(sr[e])), __uint_as_float(sr[e + 1]));
         const float t_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;  // sc > 0
         m_true = fmaxf(m_true, t_max);
-        float want = kQuant ? t_max + (v_top - kLift) : t_max - kLift;
-        if constexpr (kQuant) {
-          if (far) {  // the whole warp; S is read again, 16 columns at a time: unrolled over all, the code would slow the other tiles
-            float best = neg_inf();
-#pragma unroll 1
-            for (int c = 0; c < kCols; c += 16) {
-              uint32_t s16[16];
-              tmem_ld16(tS + col0 + c, s16);
-              tc_wait_ld();
-              const uint32_t here = (uint32_t)(mask >> (col0 + c));
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const uint32_t biased = min(max(__float_as_uint(scales[TK + c + e]) >> 23 & 0xffu, 47u), 227u);
-                const float s = __uint_as_float(s16[e]) * scales[c + e] * sc + (__uint_as_float(0x4b000000u | biased) - 8388735.f);
-                if ((here >> e) & 1u) best = fmaxf(best, s);
-              }
-            }
-            want = best - kLift;
-          }
-        }
-        const bool move = want > shift + kSlack;
+        float want = kQuant ? t_max + ((float)(min(max(v_top, 47), 227) - 127) - kLift) : t_max - kLift;
+        bool move = want > shift + kSlack;
         if (__any_sync(kFullMask, move)) {
+          if constexpr (kQuant) {  // a closer look, before it is believed
+            const volatile uint32_t* all = reinterpret_cast<const volatile uint32_t*>(scales + TK - col0);
+            const uint32_t x = all[lane] & 0x7fffffffu, y = all[lane + 32] & 0x7fffffffu;
+            const int low = (int)(__reduce_min_sync(kFullMask, min(x ? x : ~0u, y ? y : ~0u)) >> 23);  // zeros (also: no key) do not count
+            if (v_top - low > kNear) {
+              float best = neg_inf();
+#pragma unroll 1
+              for (int c = 0; c < kCols; c += 4) {
+                uint32_t s4[4];
+                tmem_ld4(tS + col0 + c, s4);
+                const float4 fk = *reinterpret_cast<const float4*>(scales + c);
+                const uint4 fv = *reinterpret_cast<const uint4*>(scales + TK + c);
+                tc_wait_ld();
+                auto one = [&](uint32_t raw, float k, uint32_t v) {
+                  const float y = fmaf(__uint_as_float(raw) * k, sc, (float)(int)(v >> 23));
+                  if (v) best = fmaxf(best, y);
+                };
+                one(s4[0], fk.x, fv.x);
+                one(s4[1], fk.y, fv.y);
+                one(s4[2], fk.z, fv.z);
+                one(s4[3], fk.w, fv.w);
+              }
+              want = fminf(fmaxf(best - 127.f, t_max - 80.f), t_max + 100.f) - kLift;
+              move = want > shift + kSlack;
+            }
+          }
           const float new_shift = move ? want : shift;
           // Scales lie up to 2^180 apart, and so do shifts, whatever the scores are: what a factor of 2^-180 leaves of l may still be most
           // of it. So the factor's root, twice.
