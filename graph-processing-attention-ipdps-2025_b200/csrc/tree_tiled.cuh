@@ -606,11 +606,12 @@ context_tiled_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_const
     // and 744.) A float16 probability times its scale is below 2^(kLift + kSlack + 1) = 2^15 then, the row's largest is at 2^4 at least
     // (native caches 2^8), and the others keep 11 bits down to 2^-18 of it and steps of 2^-28 below. Each new shift holds a warp up for
     // some 2000 cycles, and the product with it: a slack of 4 set one every fourth tile of a sequence of normal numbers.
+    // A bfloat16 probability stays below 1: V may be as large as in the kernels that compute in 32 bits.
     // What few tiles need (keys that do not exist, scales far apart) is written small, in a loop over columns that are read from tensor
     // memory again: the code of the other tiles, with that of the other roles, just fits the instruction cache. All of it in registers,
     // calls of 128 rows a unit over 8-bit caches took up to 20 % longer, with four times the cache's misses.
     constexpr bool kHalfP = std::is_same<TP, __half>::value;
-    constexpr float kSlack = kHalfP ? 6.f : 8.f, kLift = kHalfP ? 8.f : 0.f;
+    constexpr float kSlack = kHalfP ? 6.f : 8.f, kLift = kHalfP ? 8.f : -8.f;
     constexpr int kNear = 4;
     const uint64_t minus1 = pack2(-1.f, -1.f);
     constexpr uint64_t kMinusZero2 = 0x8000000080000000ull;  // x y + -0 is the product, signs of zeros included

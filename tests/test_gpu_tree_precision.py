@@ -70,3 +70,18 @@ def test_a_chunk_of_a_prompt(pkg, dtype, cache):
     for b, T in enumerate(rows):
         mask[cu[b]:cu[b + 1], :T] = torch.ones(T, T, dtype=torch.bool).tril()
     check_all(pkg, c, Q, cu, mask)
+
+
+@pytest.mark.parametrize("rows", [3, 20, 70])
+def test_bfloat16_values_near_the_largest(pkg, rows):
+    """V of 2^121 under probabilities that add up to little more than 1: finite in every kernel, whatever reference it holds them to."""
+    c, _, cu, mask = problem("bf16", "native", [900, 800, 700], [rows] * 3, 32, 16, 64, 16, "hnd", seed=rows)
+    g = torch.Generator().manual_seed(1)
+    Q = (1 + 0.1 * torch.randn(3 * rows, 32, 64, generator=g)).to(c.dtype)
+    c.K.mul_(0.02)
+    c.V.copy_(torch.where(c.V < 0, -1.0, 1.0) * (1 + c.V.abs() / 8) * 2.0 ** 121)
+    for b, n in enumerate((900, 800, 700)):  # in a later tile, scores of about 5.2: e^5.2 = 2^7.5 times the others, which are then taken away
+        for p in range(n):
+            c.K[c.place(b, p)] -= 3.0 if p % 64 else 0.0
+        c.K[c.place(b, 300)] = 0.65
+    check_all(pkg, c, Q, cu, mask)
