@@ -35,8 +35,8 @@ int check_tree(const spfa_kv_cache* c, int dtype, int64_t n_rows, int64_t n_q_he
 }
 
 // Row tiles that a CTA of the tensor-core kernel takes together: two where a sequence has more rows than one holds, on average. One
-// against two, in us: 64 tokens of 8 heads a key head over 16384 float16 / int8 keys 203 : 178, of 4 heads in bfloat16 519 : 412;
-// 8 tokens of 4 heads, 256 sequences of 512 keys, 181 : 235, 4 sequences of 8192 e4m3 keys 39 : 52.
+// against two, in us: 64 tokens of 8 heads a key head over 16384 float16 / int8 keys 236 : 169, of 4 heads in bfloat16 202 : 164;
+// 8 tokens of 4 heads, 256 sequences of 512 keys, 180 : 222, 4 sequences of 8192 e4m3 keys 39 : 52.
 int row_tiles_of(const tree::Call& a) { return a.n_rows * a.group > 128LL * a.c.n_seq ? 2 : 1; }
 
 bool tiled_call(const spfa_kv_cache* c, int dtype, const void* Q, const int64_t* Q_stride, int subs) {

@@ -175,7 +175,8 @@ struct Walk {
 // columns of O in registers and a share of the keys. Larger d leaves room for fewer keys: 4 rows x 2 keys, 4 rows x 4 columns. Pairs of
 // products share an instruction. A tile is a chain of short phases between barriers; other CTAs of the SM fill its gaps.
 // float32, 4 sequences of 16 drafted tokens, 2 heads a key head, up to 4096 keys, d = 64: 30 us with the merge, 0.8 TB/s: 2.5 tiles for a CTA,
-// so that the chain of a tile's phases counts. 64 sequences of one token over 2000 keys: 336 us, 3.1 TB/s.
+// so that the chain of a tile's phases counts. 64 sequences of one token over 2000 keys of 8 heads of 128: 520 us,
+// 2.0 TB/s.
 __host__ __device__ constexpr int any_tile_keys(int dp) { return dp <= 128 ? 64 : (dp == 256 ? 32 : 16); }
 template <int DP, int R>
 struct PlanAny {

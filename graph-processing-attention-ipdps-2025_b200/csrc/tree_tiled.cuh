@@ -21,21 +21,21 @@
 // first e4m3, the second e5m2. A row is first multiplied by a power of two that brings its largest element to [2^7, 2^8): the terms are
 // an element exactly then, down to 2^-13 of the largest (2^-6, where e4m3's subnormal numbers begin), and smaller ones are held to 2^-21
 // of it. (e4m3 alone, which ends at 2^-9, showed in l: 9e-7 of it, float32 sums 4e-7.) Without K's conversion, which passes the tile
-// through shared memory twice: 437 -> 370 us, e4m3 call below. float16 elements take three terms, and their products cost more than the
-// conversion: 491 us against 461. bfloat16 Q over int8 becomes float16 times such a power: none of its 8 bits is lost above 2^-29 of the
+// through shared memory twice: 437 -> 366 us, e4m3 call below. float16 elements take three terms, and their products cost more than the
+// conversion: 491 us against 458. bfloat16 Q over int8 becomes float16 times such a power: none of its 8 bits is lost above 2^-29 of the
 // row's largest element.
-// The rows' scales stay in fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference takes the
-// largest of them in.
+// The rows' scales stay in fp32: K's multiplies the score, V's the probability before that is rounded, and the row's reference is the
+// largest such product.
 // P is rounded to 16 bits. Where that alone would be as large as the rounding of the result (all but 8-bit caches under bfloat16 Q),
-// units of a single row tile carry a second 16-bit term, the rounding's remainder: they wait for memory, and the second product is
-// hidden. Units with more row tiles are bound by arithmetic and rows enough that the error stays at its mean, sqrt(2) of the
-// result's own rounding.
+// sequences of at most 128 rows for a key head carry a second 16-bit term, the rounding's remainder: they wait for memory, and the second
+// product is hidden. Those of more rows are bound by arithmetic, and have one: float16 over int8 is off by 3.0e-4 of the result then, with
+// two terms by 2.1e-4, the result's own rounding.
 //
 // What bounds it, on 32 sequences of up to 32768 keys, 8 tokens, 4 heads a key head (32 rows a unit), d = 128: a bfloat16 cache memory,
-// 461 us, 5.9 TB/s; e4m3 370 us, 3.8 TB/s, and int8 500 us, 2.8 TB/s, shared memory: V's (int8: K's too) way through the converting warps,
+// 460 us, 5.9 TB/s; e4m3 366 us, 3.9 TB/s, and int8 488 us, 2.9 TB/s, shared memory: V's (int8: K's too) way through the converting warps,
 // Q and the converted tiles on theirs to the tensor cores add up to its 128 bytes a cycle. Units of 256 rows are bound by the softmax
-// warps, each of which owns a row of 64 scores a tile: 403 us, 700 TFLOP/s for 64 tokens over 16384 bfloat16 keys, 175 us and 436 TFLOP/s
-// for 64 tokens of 8 heads over 16384 int8 keys under float16 Q.
+// warps, each of which owns a row of 64 scores a tile: 302 us, 910 TFLOP/s for 8 sequences of 64 tokens, 64 heads on 8, over 16384
+// bfloat16 keys; 168 us, 454 TFLOP/s for 8 of up to 64 tokens, 32 heads on 4, over up to 16384 int8 keys under float16 Q.
 #pragma once
 #include "tile_kernels_16.cuh"
 #include "tree_kernels.cuh"

@@ -445,7 +445,10 @@ int spfa_cache_keep(const spfa_kv_cache* cache, const int32_t* kept, int64_t wid
  *   - scales of an 8-bit cache are not negative and finite, at most 2^96 of K and 2^100 of V, or NaN: a NaN scale of K or V makes
  *     the rows that see it NaN. Rows above that (append holds values up to the largest of float32: scales up to 2^121) give infinities
  *     or NaN. V below 2^-71 throughout a sequence loses bits, down to zeros.
- * Everything else is computed in float32.
+ * Everything else is computed in float32: the sums of p |v| before the division by l, relative to a row's largest p, have to stay below
+ * 2^128. An infinity in V stands in its column of O with its sign in every row that sees it, both signs or a NaN make NaN; where a
+ * product is 32-bit (calls without tensor cores, drafted rows, the parts of a long row that are added up), a probability below 2^-126
+ * makes NaN of an infinity too.
  * The workspace needs spfa_tree_workspace_bytes of the same cache, n_rows and n_q_heads. */
 size_t spfa_tree_workspace_bytes(const spfa_kv_cache* cache, int dtype, int64_t n_rows, int64_t n_q_heads);
 int spfa_tree_forward(const spfa_kv_cache* cache, int dtype, const void* Q, const int64_t* Q_stride, const int32_t* cu_rows,
