@@ -85,3 +85,23 @@ def test_query_rows_that_share_their_memory(pkg, dtype, cache):
         pkg.binding("spfa_tree").forward(view, *c.args(), torch.tensor(cu, dtype=torch.int32, device="cuda"), mask.cuda(), m, l, O,
                                          *c.scales(), first=True)
         check_tree((m, l, O), want, bound, written, dim)
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "native"), ("f16", "int8")])
+def test_modules_refuse_to_write_expanded_tensors(pkg, dtype, cache):
+    c, Q, cu, mask = problem(dtype, cache, [20, 9], [3, 2], 4, 1, 64, 16)
+    c = expand(c, 2, 2)
+    mod, cu_t = pkg.binding("spfa_cache"), torch.tensor(cu, dtype=torch.int32, device="cuda")
+    rows = torch.ones(5, 2, 64, dtype=Q.dtype, device="cuda")
+    kept, before = torch.ones(2, 1, dtype=torch.int32, device="cuda"), c.K.clone()
+    m, l = (torch.zeros(5, 4, device="cuda") for _ in range(2))
+    O = torch.zeros(5, 1, 64, dtype=Q.dtype, device="cuda")
+    for bad in (lambda: mod.append(rows, rows, *c.args(), cu_t, *c.scales()), lambda: mod.keep(*c.args(), kept, kept[:, 0], *c.scales()),
+                lambda: mod.read(*c.args(), cu_t, rows[:, :1].expand(5, 2, 64), rows, *c.scales()),
+                lambda: pkg.binding("spfa_tree").forward(Q.cuda(), *c.args(), cu_t, mask.cuda(), m, l, O.expand(5, 4, 64), *c.scales())):
+        with pytest.raises(RuntimeError, match="bad argument"):
+            bad()
+    assert torch.equal(c.K.view(torch.int8 if cache == "int8" else torch.int16), before.view(torch.int8 if cache == "int8" else torch.int16))
+    assert (rows == 1).all() and not O.any()
+    mod.read(*c.args(), cu_t, rows, rows.clone(), *c.scales())  # reading from them is fine
+    assert torch.equal(rows[:, 0], rows[:, 1]) and not (rows == 1).all()
